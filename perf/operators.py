@@ -156,7 +156,16 @@ def _prepare_model(case, gen):
 
 def prepare(case, seed):
     gen = torch.Generator(device="cuda").manual_seed(seed)
-    return (_prepare_norm if case["op"].startswith("norm") else _prepare_model)(case, gen)
+    s = (_prepare_norm if case["op"].startswith("norm") else _prepare_model)(case, gen)
+    if own and case["op"].startswith("adamw"):   # the optimiser that the program keeps
+        from teenygrad_b200 import ops
+
+        state = dict(m=s["ms"], v=s["vs"]) if case["op"] == "adamw" else dict(
+            m=s["ms"], m_exp=s["m_exps"], s=s["ss"], s_exp=s["s_exps"])
+        s["plan"] = ops.AdamW(s["params"], s["grads"], lr=LR, betas=(BETA1, BETA2), eps=EPS, weight_decay=DECAY,
+                              copies=s["copies"], state_bits=32 if case["op"] == "adamw" else 8, seed=s.get("seed", 0),
+                              state=state, step_count=s["step"])
+    return s
 
 
 # ------------------------------------------------------------ plain forms ----
@@ -278,14 +287,8 @@ def run(s):
         return ops.layer_norm_backward(s["dy"], s["x"], s["w"], s["mean"], s["rstd"])
     if op == "grad_norm":
         return ops.grad_norm(s["grads"], max_norm=1.0)
-    s["step"] += 1
-    kw = dict(betas=(BETA1, BETA2), eps=EPS, weight_decay=DECAY, grad_scale=s["scale"], copies=s["copies"])
-    if op == "adamw":
-        ops.adamw_step(s["params"], s["grads"], s["ms"], s["vs"], s["step"], LR, **kw)
-        return {k: s[k] for k in ("p", "copy", "m", "v")}
-    ops.adamw8_step(s["params"], s["grads"], s["ms"], s["m_exps"], s["ss"], s["s_exps"], s["step"], LR, seed=s["seed"],
-                    **kw)
-    return {k: s[k] for k in ("p", "copy", "m", "m_exp", "s", "s_exp")}
+    s["plan"].step(grad_scale=s["scale"])
+    return {k: s[k] for k in (("p", "copy", "m", "v") if op == "adamw" else ("p", "copy", "m", "m_exp", "s", "s_exp"))}
 
 
 def work(case):
