@@ -109,7 +109,8 @@ TB_API int tb_add_fwd(tb_ctx* ctx, int dtype, const void* a, const void* b, void
 typedef enum tb_op {
     TB_OP_LINEAR = 0, TB_OP_MATMUL = 1, TB_OP_INT8_LINEAR = 2, TB_OP_RMSNORM = 3, TB_OP_LAYERNORM = 4,
     TB_OP_ACT = 5, TB_OP_ATTN = 6, TB_OP_CONV2D = 7, TB_OP_QUANTIZE_INT8 = 8,
-    TB_OP_RMSNORM_BWD = 9, TB_OP_LINEAR_BWD = 10, TB_OP_ATTN_BWD = 11, TB_OP_CONV2D_BWD = 12
+    TB_OP_RMSNORM_BWD = 9, TB_OP_LINEAR_BWD = 10, TB_OP_ATTN_BWD = 11, TB_OP_CONV2D_BWD = 12,
+    TB_OP_LAYERNORM_BWD = 13, TB_OP_GRAD_NORM = 14
 } tb_op;
 /* Row stride (elements) an executor should allocate for an op's output rows
  * of row_elems elements: RuntimeOp::forward_output_row_stride
@@ -120,7 +121,8 @@ TB_API int tb_output_row_stride(int op, int dtype, int64_t row_elems, int64_t* s
 /* Device workspace an op needs, in bytes.  shape: TB_OP_CONV2D {B, Cin,
  * Cout, H, W, KH, KW, stride, pad} (bf16 tensor-core path only);
  * TB_OP_RMSNORM_BWD {M, N}; TB_OP_LINEAR_BWD {M, N, K}; TB_OP_ATTN_BWD
- * {B, Hq, Sq}; ignored for the others (no workspace).  Needs no GPU. */
+ * {B, Hq, Sq}; TB_OP_LAYERNORM_BWD {M, N}; TB_OP_GRAD_NORM {tensors}; ignored
+ * for the others (no workspace).  Needs no GPU. */
 TB_API int tb_workspace_bytes(int op, int dtype, const int64_t* shape, int n_shape, size_t* bytes);
 
 /* ------------------------------------------------------------- linear --- */
@@ -263,6 +265,20 @@ TB_API int tb_batchnorm_fwd(tb_ctx* ctx, int dtype, const void* x, const float* 
  * (TB_OP_RMSNORM_BWD, {M, N}) when dw is given. */
 TB_API int tb_rmsnorm_bwd(tb_ctx* ctx, int dtype, const void* dy, const void* x, const void* w, const float* rrms,
                           void* dx, float* dw, int64_t M, int64_t N, void* workspace, size_t workspace_bytes);
+/* layer_norm_forward (nn/norm/layernorm.rs:163): tb_layernorm_fwd that also
+ * writes each row's mean and rstd = 1 / sqrt(var + eps) (f32 [M]), which the
+ * backward takes.  y must not overlap x, w or b.  M, N < 2^31. */
+TB_API int tb_layernorm_fwd_train(tb_ctx* ctx, int dtype, const void* x, const void* w, const void* b, void* y,
+                                  float* mean, float* rstd, int64_t M, int64_t N, float eps);
+/* Backward of layer_norm_forward: with xhat = (x - mean) rstd and a = dy w,
+ * dx[m,n] = rstd[m] (a - sum_n(a) / N - xhat sum_n(a xhat) / N),
+ * dw[n] = sum_m dy xhat, db[n] = sum_m dy (f32 [N]; added to what they hold when
+ * `accumulate` is not 0, written otherwise).  Outputs must not overlap inputs.
+ * M = 0 leaves or zeroes dw and db.  Workspace: TB_OP_LAYERNORM_BWD {M, N}, 16-byte
+ * aligned. */
+TB_API int tb_layernorm_bwd(tb_ctx* ctx, int dtype, const void* dy, const void* x, const void* w, const float* mean,
+                            const float* rstd, void* dx, float* dw, float* db, int accumulate, int64_t M, int64_t N,
+                            void* workspace, size_t workspace_bytes);
 /* linear_backward (nn/mlp/linear.rs:119-249) of y = x w^T + b: dx = dy w
  * [M, K], dw = dy^T x [N, K] (dtype; either may be NULL), db = sum_m dy
  * (f32 [N], may be NULL).  TB_BF16 on the tensor cores (M, N, K multiples of
@@ -282,6 +298,56 @@ TB_API int tb_attn_bwd(tb_ctx* ctx, int dtype, const void* q, const void* k, con
  * written (not accumulated).  KH * KW <= 49.  No workspace. */
 TB_API int tb_conv2d_bwd(tb_ctx* ctx, int dtype, const void* dy, const void* x, const void* w, void* dx, void* dw,
                          int B, int Cin, int Cout, int H, int W, int KH, int KW, int stride, int pad);
+
+/* ---------------------------------------------------------- optimiser --- */
+/* The 2-norm of all the elements of n gradient tensors (device pointers and
+ * sizes in host arrays; dtype TB_F32 or TB_BF16): norm[0] (f32, device), and, when
+ * scale is given, scale[0] = min(1, max_norm / (norm + 1e-6)), the factor that clips
+ * the gradients to max_norm (NaN for a NaN norm).  Squares are f32: one above
+ * 3.4e38 makes the norm infinite.  Sums in a fixed order.  Workspace:
+ * TB_OP_GRAD_NORM {n}, 8-byte aligned. */
+TB_API int tb_grad_norm(tb_ctx* ctx, int dtype, const void* const* grads, const int64_t* sizes, int n, float* norm,
+                        float* scale, double max_norm, void* workspace, size_t workspace_bytes);
+
+/* AdamW over many tensors (LoadedModel::adamw_step, drivers/teeny-cuda/src/
+ * model/mod.rs:868), with g' = g * grad_scale:
+ *   m = beta1 m + (1 - beta1) g'    v = beta2 v + (1 - beta2) g'^2
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps)
+ * tb_adamw_create checks the tensors once and keeps their addresses (no device
+ * memory): they must stay where they are until tb_adamw_destroy.  A step is one
+ * launch for up to 440 tensors, on the context's stream.
+ * p / g: TB_F32 / TB_F32, TB_F32 / TB_BF16 or TB_BF16 / TB_BF16; f32 parameters may
+ * have a bf16 copy that each step writes.  No tensor may overlap one that is written.
+ * state_bits 32: m and v are f32 [n].
+ * state_bits 8: m and v are e4m3 codes [n] of m and of sqrt(v), with one exponent for
+ * each 256 elements (m_exp, v_exp: uint8 [ceil(n / 256)]): value = code *
+ * 2^(exp - 127).  All zeros is the state before the first step.  New codes are rounded
+ * up or down with the probability of the rest, by a hash of (the seed's low 32 bits, t,
+ * tensor, element); a root above 0 is not rounded to 0; a moment that is not finite is
+ * stored as NaN (0x7f). */
+typedef struct tb_adamw tb_adamw;
+typedef struct tb_adamw_tensor {
+    void* p;
+    const void* g;
+    void* m;
+    void* v;
+    uint8_t* m_exp; /* state_bits 8, else NULL */
+    uint8_t* v_exp;
+    void* copy;     /* bf16 [n] or NULL */
+    int64_t n;
+} tb_adamw_tensor;
+typedef struct tb_adamw_hyper {
+    double lr, beta1, beta2, eps, weight_decay;
+    int64_t step;            /* t: 1 for the first step */
+    uint64_t seed;           /* state_bits 8 */
+    const float* lr_dev;     /* device scalars that a captured step reads at each */
+    const int64_t* step_dev; /*   replay, in place of lr and step; or NULL */
+    const float* grad_scale; /* device scalar, or NULL: 1 */
+} tb_adamw_hyper;
+TB_API int tb_adamw_create(tb_ctx* ctx, int p_dtype, int g_dtype, int state_bits, const tb_adamw_tensor* tensors, int n,
+                           tb_adamw** out);
+TB_API int tb_adamw_destroy(tb_adamw* a);
+TB_API int tb_adamw_step(tb_adamw* a, const tb_adamw_hyper* hyper);
 
 /* ------------------------------------------------------------ decoder --- */
 /* RoPE, rotate-half pairing (d, d + D/2), inv_freq = theta^(-2i/D).

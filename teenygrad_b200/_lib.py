@@ -28,6 +28,17 @@ class TeenyError(RuntimeError):
         self.status = status
 
 
+_P, _I, _L, _D, _Z = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_double, ctypes.c_size_t
+# Entry points called with plain Python numbers.
+_ARGTYPES = {
+    "tb_layernorm_fwd_train": [_P, _I, _P, _P, _P, _P, _P, _P, _L, _L, ctypes.c_float],
+    "tb_layernorm_bwd": [_P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _I, _L, _L, _P, _Z],
+    "tb_grad_norm": [_P, _I, _P, _P, _I, _P, _P, _D, _P, _Z],
+    "tb_adamw_create": [_P, _I, _I, _I, _P, _I, _P],
+    "tb_adamw_destroy": [_P],
+    "tb_adamw_step": [_P, _P],
+}
+
 _lib = None
 _lock = threading.Lock()
 
@@ -51,6 +62,8 @@ def lib() -> ctypes.CDLL:
                 l.tb_strerror.restype = ctypes.c_char_p
                 l.tb_last_error.restype = ctypes.c_char_p
                 l.tb_last_error.argtypes = [ctypes.c_void_p]
+                for name, args in _ARGTYPES.items():
+                    getattr(l, name).argtypes = args
                 _lib = l
     return _lib
 

@@ -170,6 +170,7 @@ int tb_output_row_stride(int op, int dtype, int64_t row_elems, int64_t* stride) 
         case TB_OP_LINEAR_BWD:
         case TB_OP_ATTN_BWD:
         case TB_OP_CONV2D_BWD:
+        case TB_OP_LAYERNORM_BWD:
             *stride = row_elems;   // dense rows
             return TB_OK;
         default: return TB_ERR_ARG;
@@ -200,6 +201,16 @@ int tb_workspace_bytes(int op, int dtype, const int64_t* shape, int n_shape, siz
         case TB_OP_ATTN_BWD:
         case TB_OP_CONV2D_BWD:
             return tb_backward_workspace_bytes(op, dtype, shape, n_shape, bytes);
+        case TB_OP_LAYERNORM_BWD:   // {M, N}
+            if (!shape || n_shape != 2) return TB_ERR_ARG;
+            if (shape[0] < 0 || shape[0] >= (1ll << 31) || shape[1] <= 0 || shape[1] >= (1ll << 31)) return TB_ERR_SHAPE;
+            *bytes = tb_layernorm_bwd_ws(shape[0], shape[1]);
+            return TB_OK;
+        case TB_OP_GRAD_NORM:       // {tensors}
+            if (!shape || n_shape != 1) return TB_ERR_ARG;
+            if (shape[0] < 0 || shape[0] >= (1ll << 31)) return TB_ERR_SHAPE;
+            *bytes = tb_grad_norm_ws(shape[0]);
+            return TB_OK;
         default: return TB_ERR_ARG;
     }
 }

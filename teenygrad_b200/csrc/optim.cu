@@ -1,0 +1,637 @@
+// The optimiser's side of the training step: the norm of all gradients, and
+// AdamW over many tensors in one launch with its moments in 32 bits or in 8
+// (the reference's LoadedModel::adamw_step, drivers/teeny-cuda/src/model/mod.rs:868).
+//
+//   g' = g * grad_scale        m = b1 m + (1 - b1) g'      v = b2 v + (1 - b2) g'^2
+//   p  = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)
+//
+// Bound by HBM: every value is read once and written once.  The table of tensors
+// rides in the launch's parameters, so a step copies nothing to the device, needs
+// no workspace and can be captured; the grid walks the chunks of all tensors with
+// its stride, so that small tensors share a wave and large ones are split.
+//
+// 8-bit moments.  m and s = sqrt(v) are held as e4m3 codes, one power of two a
+// block of 256 elements: value = code * 2^(exp - 127), the exponent that puts the
+// block's largest value in [128, 256).
+//  * A power of two makes the decoding exact and costs a floating code nothing.
+//  * s in place of v: its code spans 2^17 below the block's largest, as m's does,
+//    where v's would span 2^8.5 of it; and a root above zero is never stored as
+//    zero, since p's step divides by it.
+//  * b2 = 0.999 moves v by a thousandth a step, which an 8-bit code rounded to
+//    nearest never follows.  The codes are rounded up or down with the
+//    probability of the rest, by 16 bits each of a hash of (seed, step, tensor,
+//    element): the mean over the steps is the 32-bit moment's, and a run repeats.
+//  * Each operation up to the code is rounded by itself (no fused multiply-add),
+//    so the codes are defined bit for bit by the formula.
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <math.h>
+#include <stdlib.h>
+
+#include <algorithm>
+#include <new>
+
+#include "common.cuh"
+
+namespace tb {
+namespace {
+
+using bf16 = __nv_bfloat16;
+
+constexpr int kThreads = 256;
+constexpr int kChunk = 2048;      // elements of one tensor that a CTA takes at a time
+constexpr int kBlock = 256;       // elements that share an exponent: one warp, 8 a lane
+constexpr int kCtasPerSm = 4;
+
+// Tensors a launch's parameters hold: 4 KB of them cost a launch nothing, 32 KB
+// some microseconds, so models of few tensors take the small table.
+constexpr int kSmallTable = 48, kLargeTable = 440;
+
+struct Entry {
+    void* p;
+    const void* g;
+    void* m;
+    void* v;
+    uint8_t* m_exp;
+    uint8_t* v_exp;
+    void* copy;
+    int64_t n;
+};
+
+struct Hyper {
+    float lr, beta1, beta2, rest1, rest2, eps, decay, log1, log2;   // rest = 1 - beta, log = log(beta)
+    int64_t step;
+    const float* lr_dev;
+    const float* grad_scale;
+    const int64_t* step_dev;
+    uint32_t seed;
+    uint32_t first;   // number of the table's first tensor
+};
+
+template <int CAP>
+struct Table {
+    Entry e[CAP];
+    int64_t start[CAP + 1];   // first chunk of each tensor; the last entry is the number of chunks
+    uint8_t vec[CAP];         // the tensor's addresses allow vector accesses
+    int n;
+    Hyper h;
+};
+static_assert(sizeof(Table<kSmallTable>) <= 4096 - 256, "fits the small parameter space");
+static_assert(sizeof(Table<kLargeTable>) <= 32764 - 256, "fits the parameter space");
+
+// The tensor that holds a chunk, from one at or before it.
+template <int CAP>
+__device__ __forceinline__ int find(const Table<CAP>& t, int64_t chunk) {
+    int lo = 0, hi = t.n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (t.start[mid] <= chunk) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// ------------------------------------------------------------------ loads --
+__device__ __forceinline__ void load4(const float* p, float* v) {
+    const float4 a = *reinterpret_cast<const float4*>(p);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+}
+__device__ __forceinline__ void load4(const bf16* p, float* v) {
+    const uint2 a = *reinterpret_cast<const uint2*>(p);
+    v[0] = bf16_lo(a.x); v[1] = bf16_hi(a.x); v[2] = bf16_lo(a.y); v[3] = bf16_hi(a.y);
+}
+__device__ __forceinline__ void store4(float* p, const float* v) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ void store4(bf16* p, const float* v) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+}
+__device__ __forceinline__ float load1(const float* p) { return *p; }
+__device__ __forceinline__ float load1(const bf16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ void store1(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store1(bf16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+// Four elements from i of an array of n, zeros past its end.
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, int64_t i, int64_t n, bool vec, float* v) {
+    if (vec && i + 4 <= n) {
+        load4(p + i, v);
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) v[j] = i + j < n ? load1(p + i + j) : 0.f;
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* p, int64_t i, int64_t n, bool vec, const float* v) {
+    if (vec && i + 4 <= n) {
+        store4(p + i, v);
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        if (i + j < n) store1(p + i + j, v[j]);
+}
+__device__ __forceinline__ uint32_t load4(const uint8_t* p, int64_t i, int64_t n, bool vec) {
+    if (vec && i + 4 <= n) return *reinterpret_cast<const uint32_t*>(p + i);
+    uint32_t w = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        if (i + j < n) w |= (uint32_t)p[i + j] << (8 * j);
+    return w;
+}
+__device__ __forceinline__ void store4(uint8_t* p, int64_t i, int64_t n, bool vec, uint32_t w) {
+    if (vec && i + 4 <= n) {
+        *reinterpret_cast<uint32_t*>(p + i) = w;
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        if (i + j < n) p[i + j] = (uint8_t)(w >> (8 * j));
+}
+
+// ------------------------------------------------------------------ AdamW --
+// The step's scalars.
+struct Step {
+    float scale, keep, rate, root, eps;   // keep = 1 - lr wd, rate = lr / (1 - b1^t), root = 1 / sqrt(1 - b2^t)
+    uint32_t key;
+};
+
+__device__ __forceinline__ uint32_t mix(uint32_t x) {
+    // xor-shifts and odd multipliers (the fractions of sqrt 2 and sqrt 3), each a bijection
+    x ^= x >> 16;
+    x *= 0x6A09E667u;
+    x ^= x >> 15;
+    x *= 0xBB67AE85u;
+    return x ^ (x >> 16);
+}
+
+__device__ __forceinline__ Step step_of(const Hyper& h) {
+    const int64_t t = h.step_dev ? *h.step_dev : h.step;
+    const float lr = h.lr_dev ? *h.lr_dev : h.lr;
+    Step s;
+    s.scale = h.grad_scale ? *h.grad_scale : 1.f;
+    s.keep = 1.f - lr * h.decay;
+    // 1 - beta^t = -expm1(t log(beta)): no cancellation at the first steps
+    s.rate = lr / -expm1f((float)t * h.log1);
+    s.root = rsqrtf(-expm1f((float)t * h.log2));
+    s.eps = h.eps;
+    s.key = mix(mix(h.seed) ^ (uint32_t)t);
+    return s;
+}
+
+__device__ __forceinline__ float stepped(float p, float m, float root_v, const Step& s) {
+    return p * s.keep - __fdividef(s.rate * m, root_v * s.root + s.eps);
+}
+
+template <typename P, typename G, int CAP>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) adamw_kernel(const __grid_constant__ Table<CAP> t) {
+    const Step s = step_of(t.h);
+    const float b1 = t.h.beta1, b2 = t.h.beta2, r1 = t.h.rest1, r2 = t.h.rest2;
+    const int64_t chunks = t.start[t.n];
+    for (int64_t c = blockIdx.x; c < chunks; c += gridDim.x) {
+        const int k = find(t, c);
+        const Entry& e = t.e[k];
+        const bool vec = t.vec[k];
+        const int64_t n = e.n, i0 = (c - t.start[k]) * kChunk + threadIdx.x * 4;
+        P* pp = (P*)e.p;
+        const G* pg = (const G*)e.g;
+        float *pm = (float*)e.m, *pv = (float*)e.v;
+        float p[2][4], g[2][4], m[2][4], v[2][4];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int64_t i = i0 + u * (kChunk / 2);
+            if (i >= n) continue;
+            load4(pp, i, n, vec, p[u]);
+            load4(pg, i, n, vec, g[u]);
+            load4(pm, i, n, vec, m[u]);
+            load4(pv, i, n, vec, v[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int64_t i = i0 + u * (kChunk / 2);
+            if (i >= n) continue;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float gj = g[u][j] * s.scale;
+                m[u][j] = b1 * m[u][j] + r1 * gj;
+                v[u][j] = b2 * v[u][j] + r2 * gj * gj;
+                p[u][j] = stepped(p[u][j], m[u][j], sqrtf(v[u][j]), s);
+            }
+            store4(pp, i, n, vec, p[u]);
+            store4(pm, i, n, vec, m[u]);
+            store4(pv, i, n, vec, v[u]);
+            if (e.copy) store4((bf16*)e.copy, i, n, vec, p[u]);
+        }
+    }
+}
+
+// ------------------------------------------------------------ 8-bit codes --
+// 2^(e - 127) for a biased exponent, the subnormal 2^-127 among them.
+__device__ __forceinline__ float power(uint32_t e) { return __uint_as_float(e ? e << 23 : 0x00400000u); }
+
+__device__ __forceinline__ void decode4(uint32_t w, float scale, float* v) {
+    const __half2 a(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3));
+    const __half2 b(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3));
+    const float2 x = __half22float2(a), y = __half22float2(b);
+    v[0] = x.x * scale; v[1] = x.y * scale; v[2] = y.x * scale; v[3] = y.y * scale;
+}
+
+// The code's magnitude for y = |x| / scale in [0, 256) with r in (0, 2^20): the
+// 20 bits below the code's last one carry into it with probability rest / 2^20.
+// Below 2^-6 the code's steps are 2^-9 all the way down, as they are in
+// [2^-6, 2^-5), so y is moved there.
+__device__ __forceinline__ uint32_t encode(float y, uint32_t r) {
+    const bool low = y < 0.015625f;
+    const uint32_t b = __float_as_uint(low ? y + 0.015625f : y);
+    return ((b + r) >> 20) - (low ? 968u : 960u);
+}
+
+// Finite magnitudes in order; what is not finite counts as 0.
+__device__ __forceinline__ uint32_t magnitude(float x) {
+    const uint32_t u = __float_as_uint(x) & 0x7fffffffu;
+    return u < 0x7f800000u ? u : 0u;
+}
+
+__device__ __forceinline__ uint32_t exponent_of(uint32_t top) {
+    const uint32_t e = top >> 23;
+    return e > 7u ? e - 7u : 0u;
+}
+
+template <typename P, typename G, int CAP>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) adamw8_kernel(const __grid_constant__ Table<CAP> t) {
+    const Step s = step_of(t.h);
+    const float b1 = t.h.beta1, b2 = t.h.beta2, r1 = t.h.rest1, r2 = t.h.rest2;
+    const int64_t chunks = t.start[t.n];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    for (int64_t c = blockIdx.x; c < chunks; c += gridDim.x) {
+        const int k = find(t, c);
+        const Entry& e = t.e[k];
+        const bool vec = t.vec[k];
+        const int64_t n = e.n, block = (c - t.start[k]) * (kChunk / kBlock) + warp, i0 = block * kBlock;
+        if (i0 >= n) continue;   // the whole warp
+        // lane l holds elements 4 l .. 4 l + 3 of both halves of the block
+        float p[8], g[8], m[8], q[8];
+        uint32_t cm[2], cs[2];
+        const uint32_t em = e.m_exp[block], es = e.v_exp[block];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int64_t i = i0 + u * 128 + lane * 4;
+            load4((const P*)e.p, i, n, vec, p + 4 * u);
+            load4((const G*)e.g, i, n, vec, g + 4 * u);
+            cm[u] = load4((const uint8_t*)e.m, i, n, vec);
+            cs[u] = load4((const uint8_t*)e.v, i, n, vec);
+        }
+        const float dm = power(em), ds = power(es);
+        uint32_t tm = 0, ts = 0;
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            decode4(cm[u], dm, m + 4 * u);
+            decode4(cs[u], ds, q + 4 * u);
+#pragma unroll
+            for (int j = 4 * u; j < 4 * u + 4; j++) {
+                const float gj = __fmul_rn(g[j], s.scale);
+                m[j] = __fadd_rn(__fmul_rn(m[j], b1), __fmul_rn(gj, r1));
+                q[j] = __fsqrt_rn(__fadd_rn(__fmul_rn(__fmul_rn(q[j], q[j]), b2), __fmul_rn(__fmul_rn(gj, gj), r2)));
+                p[j] = stepped(p[j], m[j], q[j], s);
+                tm = max(tm, magnitude(m[j]));
+                ts = max(ts, magnitude(q[j]));
+            }
+        }
+        const uint32_t nm = exponent_of(__reduce_max_sync(0xffffffffu, tm));
+        const uint32_t ns = exponent_of(__reduce_max_sync(0xffffffffu, ts));
+        const float im = power(254u - nm), is = power(254u - ns);
+        const uint32_t key = mix(s.key ^ (t.h.first + k)) + (uint32_t)(i0 >> 32) * 0xBB67AE85u;
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int64_t i = i0 + u * 128 + lane * 4;
+            uint32_t wm = 0, ws = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float a = m[4 * u + j], b = q[4 * u + j];
+                const uint32_t bits = mix(key + ((uint32_t)i + j) * 0x9E3779B1u);
+                uint32_t x = encode(fabsf(a) * im, (bits & 0xffffu) << 4 | 8u);
+                if (x) x |= a < 0.f ? 0x80u : 0u;
+                if (!isfinite(a)) x = 0x7fu;
+                uint32_t y = encode(b * is, (bits >> 16) << 4 | 8u);
+                if (b > 0.f && !y) y = 1u;
+                if (!isfinite(b)) y = 0x7fu;
+                wm |= x << (8 * j);
+                ws |= y << (8 * j);
+            }
+            if (i < n) {
+                store4((P*)e.p, i, n, vec, p + 4 * u);
+                store4((uint8_t*)e.m, i, n, vec, wm);
+                store4((uint8_t*)e.v, i, n, vec, ws);
+                if (e.copy) store4((bf16*)e.copy, i, n, vec, p + 4 * u);
+            }
+        }
+        if (lane == 0) {
+            e.m_exp[block] = (uint8_t)nm;
+            e.v_exp[block] = (uint8_t)ns;
+        }
+    }
+}
+
+// -------------------------------------------------------------- grad norm --
+// part[blockIdx.x] = the CTA's sum of squares: f32 over a chunk's 8 elements a
+// thread, f64 over the chunks.
+template <typename G, int CAP>
+__global__ void __launch_bounds__(kThreads) sumsq_kernel(const __grid_constant__ Table<CAP> t, double* __restrict__ part) {
+    __shared__ double red[kThreads / 32];
+    const int64_t chunks = t.start[t.n];
+    double acc = 0.0;
+    for (int64_t c = blockIdx.x; c < chunks; c += gridDim.x) {
+        const int k = find(t, c);
+        const bool vec = t.vec[k];
+        const int64_t n = t.e[k].n, i0 = (c - t.start[k]) * kChunk + threadIdx.x * 4;
+        float s = 0.f;
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int64_t i = i0 + u * (kChunk / 2);
+            if (i >= n) continue;
+            float g[4];
+            load4((const G*)t.e[k].g, i, n, vec, g);
+#pragma unroll
+            for (int j = 0; j < 4; j++) s += g[j] * g[j];
+        }
+        acc += s;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x / 32] = acc;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < kThreads / 32; w++) acc += red[w];
+        part[blockIdx.x] = acc;
+    }
+}
+
+// norm = sqrt(sum of the parts), in a fixed order; scale = min(1, max_norm / (norm + 1e-6)).
+__global__ void __launch_bounds__(kThreads) norm_kernel(const double* __restrict__ part, int n, float* __restrict__ norm,
+                                                        float* __restrict__ scale, double max_norm) {
+    __shared__ double red[kThreads / 32];
+    double acc = 0.0;
+    for (int i = threadIdx.x; i < n; i += kThreads) acc += part[i];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x / 32] = acc;
+    __syncthreads();
+    if (threadIdx.x) return;
+    for (int w = 1; w < kThreads / 32; w++) acc += red[w];
+    acc = sqrt(acc);
+    *norm = (float)acc;
+    // a norm that is not a number gives a scale that is none
+    const double f = max_norm / (acc + 1e-6);
+    if (scale) *scale = f > 1.0 ? 1.f : (float)f;
+}
+
+// ------------------------------------------------------------------- host --
+int64_t chunks_of(int64_t n) { return (n + kChunk - 1) / kChunk; }
+
+// Fills a table with tensors [at, at + count) of a list; returns its chunks.
+template <int CAP>
+int64_t fill(Table<CAP>& t, const Entry* e, const uint8_t* vec, int count) {
+    t.n = count;
+    t.start[0] = 0;
+    for (int k = 0; k < count; k++) {
+        t.e[k] = e[k];
+        t.vec[k] = vec[k];
+        t.start[k + 1] = t.start[k] + chunks_of(e[k].n);
+    }
+    return t.start[count];
+}
+
+unsigned grid_for(tb_ctx* ctx, int64_t chunks) {
+    const int64_t cap = (int64_t)ctx->num_sms * kCtasPerSm;
+    return (unsigned)(chunks < cap ? chunks : cap);
+}
+
+bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+template <typename P, typename G, int CAP>
+int adamw_launch(tb_ctx* ctx, int bits, const Entry* e, const uint8_t* vec, int count, const Hyper& h) {
+    Table<CAP> t;
+    const int64_t chunks = fill(t, e, vec, count);
+    if (!chunks) return TB_OK;
+    t.h = h;
+    return launch(ctx, bits == 8 ? "adamw8" : "adamw", bits == 8 ? adamw8_kernel<P, G, CAP> : adamw_kernel<P, G, CAP>,
+                  dim3(grid_for(ctx, chunks)), dim3(kThreads), 0, t);
+}
+
+template <typename G, int CAP>
+int sumsq_launch(tb_ctx* ctx, const Entry* e, const uint8_t* vec, int count, double* part) {
+    Table<CAP> t;
+    const int64_t chunks = fill(t, e, vec, count);
+    t.h = Hyper{};
+    // every launch writes its own row of partial sums, of one CTA where there is nothing to add
+    return launch(ctx, "grad_norm", sumsq_kernel<G, CAP>, dim3(chunks ? grid_for(ctx, chunks) : 1u), dim3(kThreads), 0, t,
+                  part);
+}
+
+int launches_of(int n) { return n <= kSmallTable ? 1 : (n + kLargeTable - 1) / kLargeTable; }
+
+}  // namespace
+}  // namespace tb
+
+using namespace tb;
+
+struct tb_adamw {
+    tb_ctx* ctx = nullptr;
+    int p_dtype = 0, g_dtype = 0, bits = 32, n = 0;
+    Entry* e = nullptr;
+    uint8_t* vec = nullptr;
+};
+
+namespace tb {
+namespace {
+
+struct Range {
+    uintptr_t lo, hi;
+    bool written;
+};
+
+// Whether two ranges meet of which one is written.
+bool overlap(Range* r, size_t n) {
+    std::sort(r, r + n, [](const Range& a, const Range& b) { return a.lo < b.lo; });
+    uintptr_t written = 0, any = 0;
+    for (size_t i = 0; i < n; i++) {
+        if (r[i].lo < (r[i].written ? any : written)) return true;
+        any = std::max(any, r[i].hi);
+        if (r[i].written) written = std::max(written, r[i].hi);
+    }
+    return false;
+}
+
+}  // namespace
+}  // namespace tb
+
+extern "C" {
+
+int tb_adamw_create(tb_ctx* ctx, int p_dtype, int g_dtype, int state_bits, const tb_adamw_tensor* tensors, int n,
+                    tb_adamw** out) {
+    if (!out) return TB_ERR_ARG;
+    *out = nullptr;
+    if (!ctx) return TB_ERR_ARG;
+    TB_REQUIRE(ctx, n >= 0 && (n == 0 || tensors), TB_ERR_ARG, "adamw: bad list of tensors");
+    const bool types = (p_dtype == TB_F32 && (g_dtype == TB_F32 || g_dtype == TB_BF16)) ||
+                       (p_dtype == TB_BF16 && g_dtype == TB_BF16);
+    TB_REQUIRE(ctx, types, TB_ERR_UNSUPPORTED, "adamw: parameters and gradients f32 / f32, f32 / bf16 or bf16 / bf16");
+    TB_REQUIRE(ctx, state_bits == 32 || state_bits == 8, TB_ERR_UNSUPPORTED, "adamw: moments in 32 or 8 bits");
+    const size_t ps = p_dtype == TB_F32 ? 4 : 2, gs = g_dtype == TB_F32 ? 4 : 2, ms = state_bits / 8;
+    for (int k = 0; k < n; k++) {
+        const tb_adamw_tensor& t = tensors[k];
+        TB_REQUIRE(ctx, t.n >= 0 && t.n < (1ll << 48), TB_ERR_SHAPE, "adamw: tensor %d has %lld elements", k, (long long)t.n);
+        if (!t.n) continue;
+        TB_REQUIRE(ctx, t.p && t.g && t.m && t.v && (state_bits == 32 || (t.m_exp && t.v_exp)), TB_ERR_ARG,
+                   "adamw: null pointer in tensor %d", k);
+        TB_REQUIRE(ctx, aligned(t.p, ps) && aligned(t.g, gs) && aligned(t.m, ms) && aligned(t.v, ms) &&
+                            aligned(t.copy, 2),
+                   TB_ERR_ALIGN, "adamw: tensor %d is not aligned to its type", k);
+        TB_REQUIRE(ctx, !t.copy || p_dtype == TB_F32, TB_ERR_UNSUPPORTED, "adamw: a bf16 copy goes with f32 parameters");
+    }
+    tb_adamw* a = new (std::nothrow) tb_adamw();
+    Range* r = (Range*)malloc(sizeof(Range) * 7 * (size_t)(n + 1));
+    if (a) {
+        a->e = (Entry*)malloc(sizeof(Entry) * (size_t)(n + 1));
+        a->vec = (uint8_t*)malloc((size_t)(n + 1));
+    }
+    if (!a || !r || !a->e || !a->vec) {
+        free(r);
+        tb_adamw_destroy(a);
+        return set_error(ctx, TB_ERR_OOM, "adamw: out of host memory");
+    }
+    a->ctx = ctx;
+    a->p_dtype = p_dtype;
+    a->g_dtype = g_dtype;
+    a->bits = state_bits;
+    a->n = n;
+    size_t nr = 0;
+    auto add = [&](const void* p, size_t bytes, bool written) {
+        if (p && bytes) r[nr++] = {(uintptr_t)p, (uintptr_t)p + bytes, written};
+    };
+    for (int k = 0; k < n; k++) {
+        const tb_adamw_tensor& t = tensors[k];
+        a->e[k] = {t.p, t.g, t.m, t.v, t.m_exp, t.v_exp, t.copy, t.n};
+        a->vec[k] = aligned(t.p, 4 * ps) && aligned(t.g, 4 * gs) && aligned(t.m, 4 * ms) && aligned(t.v, 4 * ms) &&
+                    aligned(t.copy, 8);
+        const size_t cnt = (size_t)t.n, blocks = (cnt + kBlock - 1) / kBlock;
+        add(t.p, cnt * ps, true);
+        add(t.g, cnt * gs, false);
+        add(t.m, cnt * ms, true);
+        add(t.v, cnt * ms, true);
+        add(t.copy, cnt * 2, true);
+        if (state_bits == 8) {
+            add(t.m_exp, blocks, true);
+            add(t.v_exp, blocks, true);
+        }
+    }
+    const bool bad = overlap(r, nr);
+    free(r);
+    if (bad) {
+        tb_adamw_destroy(a);
+        return set_error(ctx, TB_ERR_ARG, "adamw: tensors overlap (a parameter listed twice, or memory shared)");
+    }
+    *out = a;
+    return TB_OK;
+}
+
+int tb_adamw_destroy(tb_adamw* a) {
+    if (!a) return TB_OK;
+    free(a->e);
+    free(a->vec);
+    delete a;
+    return TB_OK;
+}
+
+int tb_adamw_step(tb_adamw* a, const tb_adamw_hyper* hy) {
+    if (!a) return TB_ERR_ARG;
+    tb_ctx* ctx = a->ctx;
+    TB_REQUIRE(ctx, hy, TB_ERR_ARG, "adamw: null pointer");
+    // written so that a NaN fails each of them
+    TB_REQUIRE(ctx, hy->beta1 >= 0 && hy->beta1 < 1 && hy->beta2 >= 0 && hy->beta2 < 1 && hy->eps >= 0 &&
+                        hy->weight_decay >= 0 && (hy->lr_dev || hy->lr >= 0),
+               TB_ERR_ARG, "adamw: betas in [0, 1), lr, eps and weight_decay >= 0");
+    TB_REQUIRE(ctx, hy->step_dev || hy->step >= 1, TB_ERR_ARG, "adamw: steps count from 1");
+    TB_REQUIRE(ctx, aligned(hy->lr_dev, 4) && aligned(hy->grad_scale, 4) && aligned(hy->step_dev, 8), TB_ERR_ALIGN,
+               "adamw: a scalar is not aligned to its type");
+    Hyper h = {};
+    h.lr = (float)hy->lr;
+    h.beta1 = (float)hy->beta1;
+    h.beta2 = (float)hy->beta2;
+    h.rest1 = (float)(1.0 - hy->beta1);
+    h.rest2 = (float)(1.0 - hy->beta2);
+    h.eps = (float)hy->eps;
+    h.decay = (float)hy->weight_decay;
+    h.log1 = (float)log(hy->beta1);   // -inf for 0: the correction is 1
+    h.log2 = (float)log(hy->beta2);
+    h.step = hy->step;
+    h.lr_dev = hy->lr_dev;
+    h.grad_scale = hy->grad_scale;
+    h.step_dev = hy->step_dev;
+    h.seed = (uint32_t)hy->seed;
+    const int cap = a->n <= kSmallTable ? kSmallTable : kLargeTable;
+    for (int at = 0; at < a->n; at += cap) {
+        const int count = std::min(cap, a->n - at);
+        h.first = (uint32_t)at;
+        auto go = [&](auto small, auto large) {
+            return cap == kSmallTable ? small(ctx, a->bits, a->e + at, a->vec + at, count, h)
+                                      : large(ctx, a->bits, a->e + at, a->vec + at, count, h);
+        };
+        const int rc = a->p_dtype == TB_BF16   ? go(adamw_launch<bf16, bf16, kSmallTable>, adamw_launch<bf16, bf16, kLargeTable>)
+                       : a->g_dtype == TB_BF16 ? go(adamw_launch<float, bf16, kSmallTable>, adamw_launch<float, bf16, kLargeTable>)
+                                               : go(adamw_launch<float, float, kSmallTable>, adamw_launch<float, float, kLargeTable>);
+        if (rc) return rc;
+    }
+    return TB_OK;
+}
+
+size_t tb_grad_norm_ws(int64_t n) {
+    // a row of partial sums for each launch: CTAs for 160 SMs
+    return n < 0 || n >= (1ll << 31) ? 0 : (size_t)launches_of((int)n) * 160 * kCtasPerSm * 8;
+}
+
+int tb_grad_norm(tb_ctx* ctx, int dtype, const void* const* grads, const int64_t* sizes, int n, float* norm, float* scale,
+                 double max_norm, void* workspace, size_t workspace_bytes) {
+    if (!ctx) return TB_ERR_ARG;
+    TB_REQUIRE(ctx, n >= 0 && (n == 0 || (grads && sizes)) && norm, TB_ERR_ARG, "grad_norm: null pointer");
+    if (dtype != TB_F32 && dtype != TB_BF16) return set_error(ctx, TB_ERR_UNSUPPORTED, "grad_norm: dtype %d", dtype);
+    TB_REQUIRE(ctx, !scale || max_norm >= 0, TB_ERR_ARG, "grad_norm: max_norm >= 0");
+    const size_t es = dtype == TB_F32 ? 4 : 2;
+    for (int k = 0; k < n; k++) {
+        TB_REQUIRE(ctx, sizes[k] >= 0 && sizes[k] < (1ll << 48), TB_ERR_SHAPE, "grad_norm: tensor %d has %lld elements", k,
+                   (long long)sizes[k]);
+        TB_REQUIRE(ctx, grads[k] || !sizes[k], TB_ERR_ARG, "grad_norm: null pointer");
+        TB_REQUIRE(ctx, aligned(grads[k], es), TB_ERR_ALIGN, "grad_norm: tensor %d is not aligned to its type", k);
+    }
+    const size_t need = tb_grad_norm_ws(n);
+    TB_REQUIRE(ctx, workspace && workspace_bytes >= need && aligned(workspace, 8), TB_ERR_ARG,
+               "grad_norm: workspace of %zu bytes required (tb_workspace_bytes)", need);
+    TB_REQUIRE(ctx, ctx->num_sms <= 160, TB_ERR_UNSUPPORTED, "grad_norm: more SMs than the workspace is made for");
+    double* part = (double*)workspace;
+    const int cap = n <= kSmallTable ? kSmallTable : kLargeTable;
+    int parts = 0;
+    for (int at = 0; at < n || at == 0; at += cap) {
+        const int count = std::min(cap, n - at);
+        Entry e[kLargeTable];
+        uint8_t vec[kLargeTable];
+        int64_t chunks = 0;
+        for (int k = 0; k < count; k++) {
+            e[k] = Entry{};
+            e[k].g = grads[at + k];
+            e[k].n = sizes[at + k];
+            vec[k] = aligned(e[k].g, 4 * es);
+            chunks += chunks_of(e[k].n);
+        }
+        auto go = [&](auto small, auto large) {
+            return cap == kSmallTable ? small(ctx, e, vec, count, part + parts) : large(ctx, e, vec, count, part + parts);
+        };
+        const int rc = dtype == TB_F32 ? go(sumsq_launch<float, kSmallTable>, sumsq_launch<float, kLargeTable>)
+                                       : go(sumsq_launch<bf16, kSmallTable>, sumsq_launch<bf16, kLargeTable>);
+        if (rc) return rc;
+        parts += chunks ? (int)grid_for(ctx, chunks) : 1;
+    }
+    return launch(ctx, "grad_norm_final", norm_kernel, dim3(1), dim3(kThreads), 0, (const double*)part, parts, norm, scale,
+                  max_norm);
+}
+
+}  // extern "C"

@@ -69,6 +69,40 @@ _i64 = ctypes.c_int64
 _f = ctypes.c_float
 
 
+class _on:
+    """The context of a device, which is the current one inside the block."""
+
+    __slots__ = ("device", "back")
+
+    def __init__(self, device):
+        self.device = device
+
+    def __enter__(self):
+        self.back = torch.cuda.current_device()
+        if self.back != self.device:
+            torch.cuda.set_device(self.device)
+        return context(self.device)
+
+    def __exit__(self, *exc):
+        if self.back != self.device:
+            torch.cuda.set_device(self.back)
+
+
+def _same(*ts):
+    """The one device that the tensors are on."""
+    devices = {t.get_device() for t in ts if t is not None}
+    if len(devices) > 1:
+        raise TeenyError(1, "tensors must be on one device")
+    return devices.pop()
+
+
+def _columns(N, dtype, *ts):
+    for t in ts:
+        if t.dtype != dtype or t.numel() != N:
+            raise TeenyError(2, f"expected {N} elements of {dtype}, got {tuple(t.shape)} of {t.dtype}")
+
+
+
 # --------------------------------------------------------------- norms ----
 def rms_norm(x, w, eps=1e-8, return_rrms=False):
     """rms_norm_forward (nn/norm/rmsnorm.rs:40-122); x [..., N]."""
@@ -82,11 +116,22 @@ def rms_norm(x, w, eps=1e-8, return_rrms=False):
     return (y, rrms) if return_rrms else y
 
 
-def layer_norm(x, w, b, eps=1e-5):
-    """layer_norm_forward_inference (nn/norm/layernorm.rs:43-157)."""
+def layer_norm(x, w, b, eps=1e-5, return_stats=False):
+    """layer_norm_forward_inference (nn/norm/layernorm.rs:43-157); with
+    return_stats=True layer_norm_forward (:163): (y, mean, rstd), the row
+    statistics f32 [M] that layer_norm_backward takes."""
     _cuda(x, w, b)
     N = x.shape[-1]
     y = torch.empty_like(x)
+    if return_stats:
+        dev = _same(x, w, b)
+        _columns(N, x.dtype, w, b)
+        M = x.numel() // N
+        mean, rstd = torch.empty(2, M, device=x.device, dtype=torch.float32)
+        with _on(dev) as ctx:
+            check(ctx, lib().tb_layernorm_fwd_train(ctx, _dt(x), x.data_ptr(), w.data_ptr(), b.data_ptr(), y.data_ptr(),
+                                                    mean.data_ptr(), rstd.data_ptr(), M, N, eps))
+        return y, mean, rstd
     ctx = context()
     check(ctx, lib().tb_layernorm_fwd(ctx, _dt(x), _p(x), _p(w), _p(b), _p(y), _i64(x.numel() // N), _i64(N), _f(eps)))
     return y
@@ -458,7 +503,8 @@ def _workspace(op, dtype, shape, device):
     return torch.empty(max(n.value, 16), dtype=torch.uint8, device=device), n.value
 
 
-TB_OP.update({"rmsnorm_bwd": 9, "linear_bwd": 10, "attn_bwd": 11, "conv2d_bwd": 12})
+TB_OP.update({"rmsnorm_bwd": 9, "linear_bwd": 10, "attn_bwd": 11, "conv2d_bwd": 12, "layernorm_bwd": 13,
+              "grad_norm": 14})
 
 
 def rms_norm_backward(dy, x, w, rrms, dw=None):
@@ -475,6 +521,34 @@ def rms_norm_backward(dy, x, w, rrms, dw=None):
     check(ctx, lib().tb_rmsnorm_bwd(ctx, _dt(x), _p(dy), _p(x), _p(w), _p(rrms), _p(dx), _p(dw), _i64(M), _i64(N),
                                     _p(ws), ctypes.c_size_t(nb)))
     return dx, dw
+
+
+def layer_norm_backward(dy, x, w, mean, rstd, dw=None, db=None):
+    """Backward of layer_norm_forward (nn/norm/layernorm.rs:163): returns (dx, dw, db)
+    from the forward's mean and rstd (f32 [M]); dw and db (f32 [N]) accumulate into
+    the given tensors (both or neither)."""
+    _cuda(dy, x, w, mean, rstd, dw, db)
+    dev = _same(dy, x, w, mean, rstd, dw, db)
+    N = x.shape[-1]
+    M = x.numel() // N
+    if dy.shape != x.shape or dy.dtype != x.dtype:
+        raise TeenyError(2, f"dy is {tuple(dy.shape)} of {dy.dtype}, x {tuple(x.shape)} of {x.dtype}")
+    if (dw is None) != (db is None):
+        raise TeenyError(1, "give both of dw and db, or neither")
+    _columns(N, x.dtype, w)
+    _columns(M, torch.float32, mean, rstd)
+    accumulate = dw is not None
+    if accumulate:
+        _columns(N, torch.float32, dw, db)
+    else:
+        dw, db = torch.empty(2, N, device=x.device, dtype=torch.float32)
+    dx = torch.empty_like(x)
+    ws, nb = _workspace("layernorm_bwd", _dt(x), (M, N), x.device)
+    with _on(dev) as ctx:
+        check(ctx, lib().tb_layernorm_bwd(ctx, _dt(x), dy.data_ptr(), x.data_ptr(), w.data_ptr(), mean.data_ptr(),
+                                          rstd.data_ptr(), dx.data_ptr(), dw.data_ptr(), db.data_ptr(), accumulate, M, N,
+                                          ws.data_ptr(), nb))
+    return dx, dw, db
 
 
 def linear_backward(x, w, dy, bias=True):
@@ -521,3 +595,161 @@ def conv2d_backward(dy, x, w, stride=1, pad=0):
                                    ctypes.c_int(Cin), ctypes.c_int(Cout), ctypes.c_int(H), ctypes.c_int(W),
                                    ctypes.c_int(KH), ctypes.c_int(KW), ctypes.c_int(stride), ctypes.c_int(pad)))
     return dx, dw
+
+
+# -------------------------------------------------------------- optimiser ---
+def _listed(what, ts, numel=None):
+    """Checks a list of tensors of one type and device; returns that type, the sizes and the addresses."""
+    for t in ts:
+        if not t.is_cuda:
+            raise TeenyError(1, "tensors must be on a CUDA device (no CPU fallback)")
+        if not t.is_contiguous():
+            raise TeenyError(2, "tensors must be contiguous")
+    if len({t.dtype for t in ts}) > 1:
+        raise TeenyError(5, f"{what} must have one dtype")
+    sizes = [t.numel() for t in ts]
+    if numel is not None and sizes != numel:
+        raise TeenyError(2, f"{what} must match the parameters, tensor by tensor")
+    return ts[0].dtype if ts else None, sizes, [t.data_ptr() for t in ts]
+
+
+def grad_norm(grads, max_norm=None):
+    """The 2-norm over all the tensors of a list (f32 [1], on the device); with max_norm
+    (norm, scale), scale = min(1, max_norm / (norm + 1e-6)) being what AdamW.step takes as
+    grad_scale to clip the gradients to max_norm."""
+    grads = list(grads)
+    dtype, sizes, ptrs = _listed("gradients", grads)
+    dev = _same(*grads) if grads else torch.cuda.current_device()
+    if grads and dtype not in _DT:
+        raise TeenyError(5, f"unsupported dtype {dtype}")
+    n = len(grads)
+    out = torch.empty(2, device=torch.device("cuda", dev), dtype=torch.float32)
+    ws, nb = _workspace("grad_norm", TB_F32, (n,), out.device)
+    at = out.data_ptr()
+    with _on(dev) as ctx:
+        check(ctx, lib().tb_grad_norm(ctx, _DT.get(dtype, TB_F32), (ctypes.c_uint64 * n)(*ptrs),
+                                      (ctypes.c_int64 * n)(*sizes), n, at, None if max_norm is None else at + 4,
+                                      0.0 if max_norm is None else max_norm, ws.data_ptr(), nb))
+    return out[:1] if max_norm is None else (out[:1], out[1:])
+
+
+class _AdamWHyper(ctypes.Structure):
+    _fields_ = [("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double),
+                ("eps", ctypes.c_double), ("weight_decay", ctypes.c_double), ("step", ctypes.c_int64),
+                ("seed", ctypes.c_uint64), ("lr_dev", ctypes.c_void_p), ("step_dev", ctypes.c_void_p),
+                ("grad_scale", ctypes.c_void_p)]
+
+
+class AdamW:
+    """LoadedModel::adamw_step (drivers/teeny-cuda/src/model/mod.rs:868) over many tensors in one
+    launch (tb_adamw_step):
+
+        g = grad * grad_scale;  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2
+        p = p (1 - lr weight_decay) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
+
+    params and grads: lists of contiguous CUDA tensors, f32 / f32, f32 / bf16 or bf16 / bf16;
+    copies: bf16 tensors that get each step's f32 parameters.  The addresses are kept: step() refuses
+    to run once a tensor has been given other memory.  Tensors must not overlap.
+
+    state_bits=32: m and v are f32.  state_bits=8: m and s = sqrt(v) are float8_e4m3fn with a uint8
+    exponent for each 256 elements (m_exp, s_exp): code * 2^(exp - 127), rounded up or down at random
+    by a hash of seed, step, tensor and element.  The lists are attributes (m, v, or m, m_exp, s,
+    s_exp); `state`, a dict of such lists, continues from them, in place, as step_count does.
+
+    capturable=True keeps the step count on the device, so that a captured step counts on at each
+    replay; an lr given as a number is then the one of the capture, one given as an f32 CUDA tensor
+    of one element is read at each replay.  Without it a step cannot be captured."""
+
+    def __init__(self, params, grads, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32,
+                 copies=None, seed=0, state=None, step_count=0, capturable=False):
+        self._handle = None
+        self.params, self.grads = list(params), list(grads)
+        self.copies = None if copies is None else list(copies)
+        self.lr, self.state_bits = lr, state_bits
+        if state_bits not in (8, 32):
+            raise TeenyError(5, "moments in 32 or 8 bits")
+        if step_count < 0:
+            raise TeenyError(1, "step_count must not be negative")
+        pd, sizes, pp = _listed("parameters", self.params)
+        gd, _, gp = _listed("gradients", self.grads, sizes)
+        n = len(sizes)
+        blocks = [-(-k // 256) for k in sizes]
+        names = (("m", torch.float32, sizes), ("v", torch.float32, sizes)) if state_bits == 32 else (
+            ("m", torch.float8_e4m3fn, sizes), ("s", torch.float8_e4m3fn, sizes), ("m_exp", torch.uint8, blocks),
+            ("s_exp", torch.uint8, blocks))
+        ptrs = []
+        for name, dtype, want in names:
+            if state is None:
+                ts = [torch.zeros(k, device=p.device, dtype=torch.uint8 if state_bits == 8 else dtype)
+                      for k, p in zip(want, self.params)]
+                ts = [t.view(dtype) for t in ts]
+            else:
+                ts = list(state[name])
+            d, _, at = _listed(name, ts, want)
+            if n and d != dtype:
+                raise TeenyError(5, f"{name} must be {dtype}, got {d}")
+            setattr(self, name, ts)
+            ptrs.append(at)
+        cp = [0] * n
+        if self.copies is not None:
+            cd, _, cp = _listed("copies", self.copies, sizes)
+            if n and cd != torch.bfloat16:
+                raise TeenyError(5, f"copies must be bfloat16, got {cd}")
+        if n and (pd not in _DT or gd not in _DT):
+            raise TeenyError(5, f"unsupported dtypes {pd}, {gd}")
+        lists = [self.params, self.grads, self.copies or []] + [getattr(self, name) for name, _, _ in names]
+        self.device = _same(*(t for ts in lists for t in ts)) if n else torch.cuda.current_device()
+        exps = ptrs[2:] or [[0] * n, [0] * n]
+        rows = (ctypes.c_uint64 * (8 * n))(*(f for row in zip(pp, gp, ptrs[0], ptrs[1], *exps, cp, sizes) for f in row))
+        # the memory lives as long as the optimiser, whatever becomes of the tensors
+        self._alive = [t.detach() for ts in lists for t in ts]
+        self._watched, self._at = [t for ts in lists for t in ts], [t.data_ptr() for t in self._alive]
+        self._hyper = _AdamWHyper(0.0, betas[0], betas[1], eps, weight_decay, 0, seed & 0xFFFFFFFF, None, None, None)
+        self._step_dev, self._step = None, step_count
+        if capturable:
+            self._step_dev = torch.full((1,), step_count, device=torch.device("cuda", self.device), dtype=torch.int64)
+            self._hyper.step_dev = self._step_dev.data_ptr()
+        if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1 and eps >= 0 and weight_decay >= 0):
+            raise TeenyError(1, "betas in [0, 1), eps and weight_decay >= 0")
+        self._handle = ctypes.c_void_p()
+        with _on(self.device) as ctx:
+            check(ctx, lib().tb_adamw_create(ctx, _DT.get(pd, TB_F32), _DT.get(gd, TB_F32), state_bits, rows, n,
+                                             ctypes.byref(self._handle)))
+
+    def __del__(self):
+        if getattr(self, "_handle", None):
+            lib().tb_adamw_destroy(self._handle)
+            self._handle = None
+
+    @property
+    def step_count(self):
+        """Steps taken (waits for the device when capturable)."""
+        return self._step if self._step_dev is None else int(self._step_dev)
+
+    def _scalar(self, what, t):
+        if not t.is_cuda or t.dtype != torch.float32 or t.numel() != 1 or t.get_device() != self.device:
+            raise TeenyError(1, f"{what}: an f32 tensor of one element on the parameters' device")
+        return t.data_ptr()
+
+    def step(self, lr=None, grad_scale=None):
+        """One step, on the current stream.  lr: a number, or an f32 CUDA tensor of one element (default:
+        self.lr).  grad_scale: such a tensor, which multiplies the gradients."""
+        lr = self.lr if lr is None else lr
+        h = self._hyper
+        if [t.data_ptr() for t in self._watched] != self._at:
+            raise TeenyError(1, "a tensor has been given other memory: make a new AdamW with this one's state")
+        if isinstance(lr, torch.Tensor):
+            h.lr, h.lr_dev = 0.0, self._scalar("lr", lr)
+        elif lr >= 0:
+            h.lr, h.lr_dev = lr, None
+        else:
+            raise TeenyError(1, f"lr must not be negative, got {lr}")
+        h.grad_scale = None if grad_scale is None else self._scalar("grad_scale", grad_scale)
+        with _on(self.device) as ctx:
+            if self._step_dev is not None:
+                self._step_dev.add_(1)
+            elif torch.cuda.is_current_stream_capturing():
+                raise TeenyError(5, "a step whose count is on the host cannot be captured: AdamW(capturable=True)")
+            h.step = self._step + 1
+            check(ctx, lib().tb_adamw_step(self._handle, ctypes.byref(h)))
+            self._step += 1
