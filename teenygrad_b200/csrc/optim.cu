@@ -40,6 +40,7 @@ using bf16 = __nv_bfloat16;
 
 constexpr int kThreads = 256;
 constexpr int kChunk = 2048;      // elements of one tensor that a CTA takes at a time
+constexpr int kNormChunk = 8192;  // the same of the gradient norm
 constexpr int kBlock = 256;       // elements that share an exponent: one warp, 8 a lane
 constexpr int kCtasPerSm = 4;
 
@@ -79,7 +80,7 @@ struct Table {
 static_assert(sizeof(Table<kSmallTable>) <= 4096 - 256, "fits the small parameter space");
 static_assert(sizeof(Table<kLargeTable>) <= 32764 - 256, "fits the parameter space");
 
-// The tensor that holds a chunk, from one at or before it.
+// The tensor that holds a chunk.
 template <int CAP>
 __device__ __forceinline__ int find(const Table<CAP>& t, int64_t chunk) {
     int lo = 0, hi = t.n;
@@ -89,6 +90,14 @@ __device__ __forceinline__ int find(const Table<CAP>& t, int64_t chunk) {
         else hi = mid;
     }
     return lo;
+}
+
+// The same for a chunk at or after one that tensor k holds: the grid's stride passes
+// few tensors at a time.
+template <int CAP>
+__device__ __forceinline__ int advance(const Table<CAP>& t, int k, int64_t chunk) {
+    while (t.start[k + 1] <= chunk) k++;
+    return k;
 }
 
 // ------------------------------------------------------------------ loads --
@@ -179,8 +188,11 @@ __device__ __forceinline__ Step step_of(const Hyper& h) {
     return s;
 }
 
+// The quotient has 2 units in the last place; a numerator under 2^-126 counts as 0.
 __device__ __forceinline__ float stepped(float p, float m, float root_v, const Step& s) {
-    return p * s.keep - __fdividef(s.rate * m, root_v * s.root + s.eps);
+    float q;
+    asm("div.approx.ftz.f32 %0, %1, %2;" : "=f"(q) : "f"(s.rate * m), "f"(root_v * s.root + s.eps));
+    return p * s.keep - q;
 }
 
 template <typename P, typename G, int CAP>
@@ -188,8 +200,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) adamw_kernel(const __gri
     const Step s = step_of(t.h);
     const float b1 = t.h.beta1, b2 = t.h.beta2, r1 = t.h.rest1, r2 = t.h.rest2;
     const int64_t chunks = t.start[t.n];
+    int k = find(t, blockIdx.x);
     for (int64_t c = blockIdx.x; c < chunks; c += gridDim.x) {
-        const int k = find(t, c);
+        k = advance(t, k, c);
         const Entry& e = t.e[k];
         const bool vec = t.vec[k];
         const int64_t n = e.n, i0 = (c - t.start[k]) * kChunk + threadIdx.x * 4;
@@ -226,8 +239,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) adamw_kernel(const __gri
 }
 
 // ------------------------------------------------------------ 8-bit codes --
-// 2^(e - 127) for a biased exponent, the subnormal 2^-127 among them.
-__device__ __forceinline__ float power(uint32_t e) { return __uint_as_float(e ? e << 23 : 0x00400000u); }
+// 2^e for e in [-149, 127], exact.
+__device__ __forceinline__ float power(int e) {
+    return __uint_as_float(e >= -126 ? (uint32_t)(e + 127) << 23 : 1u << (e + 149));
+}
 
 __device__ __forceinline__ void decode4(uint32_t w, float scale, float* v) {
     const __half2 a(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3));
@@ -236,123 +251,198 @@ __device__ __forceinline__ void decode4(uint32_t w, float scale, float* v) {
     v[0] = x.x * scale; v[1] = x.y * scale; v[2] = y.x * scale; v[3] = y.y * scale;
 }
 
-// The code's magnitude for y = |x| / scale in [0, 256) with r in (0, 2^20): the
-// 20 bits below the code's last one carry into it with probability rest / 2^20.
-// Below 2^-6 the code's steps are 2^-9 all the way down, as they are in
-// [2^-6, 2^-5), so y is moved there.
-__device__ __forceinline__ uint32_t encode(float y, uint32_t r) {
-    const bool low = y < 0.015625f;
-    const uint32_t b = __float_as_uint(low ? y + 0.015625f : y);
-    return ((b + r) >> 20) - (low ? 968u : 960u);
-}
-
-// Finite magnitudes in order; what is not finite counts as 0.
-__device__ __forceinline__ uint32_t magnitude(float x) {
-    const uint32_t u = __float_as_uint(x) & 0x7fffffffu;
-    return u < 0x7f800000u ? u : 0u;
-}
-
 __device__ __forceinline__ uint32_t exponent_of(uint32_t top) {
     const uint32_t e = top >> 23;
     return e > 7u ? e - 7u : 0u;
 }
 
+// Codes.  x is scaled to put the code's smallest normal value, 2^-6, on f32's, 2^-126: then
+// the code is the f32's bits 20 to 26, in the subnormal range too, and what lies below them
+// carries into it with probability rest / 2^20 when 16 random bits (and a half) are added.
+constexpr int kCodeScale = -120;
+
+__device__ __forceinline__ uint32_t random_m(uint32_t bits) { return (bits << 4 & 0xffff0u) + 8u; }
+__device__ __forceinline__ uint32_t random_s(uint32_t bits) { return (bits >> 12 & 0xffff0u) + 8u; }
+
+// What is above zero keeps a code above zero.
+__device__ __forceinline__ uint32_t above_zero(uint32_t t, float x) { return x > 0.f ? max(t, 1u << 20) : t; }
+
+// Bytes 3 of four words.
+__device__ __forceinline__ uint32_t top_bytes(const uint32_t* t) {
+    return __byte_perm(__byte_perm(t[0], t[1], 0x0073), __byte_perm(t[2], t[3], 0x7300), 0x7610);
+}
+
+// A block with a value that is not finite (it becomes NaN, and does not count for the block's
+// exponent) or with an exponent too large for one factor: the scaling in two.
+__device__ __noinline__ uint32_t odd_code(float x, uint32_t e, uint32_t r, bool root) {
+    if (!isfinite(x)) return 0x7fu;
+    uint32_t t = __float_as_uint(fabsf(x) * power(127 - (int)e) * power(kCodeScale)) + r;
+    if (root) t = above_zero(t, x);
+    return t >> 20 | (root ? 0u : __float_as_uint(x) >> 24 & 0x80u);
+}
+__device__ __forceinline__ uint32_t finite_bits(float x) {
+    const uint32_t u = __float_as_uint(x) & 0x7fffffffu;
+    return u < 0x7f800000u ? u : 0u;
+}
+
+// One block of 256 elements from i0 of tensor e, by a warp: lane l has elements 4 l .. 4 l + 3
+// of both halves.  FULL: all of them exist, and their addresses allow vectors.
+template <typename P, typename G, bool FULL>
+__device__ __forceinline__ void adamw8_block(const Entry& e, int64_t block, bool vec, const Hyper& h, const Step& s,
+                                             uint32_t key) {
+    const int lane = threadIdx.x & 31;
+    const int64_t n = e.n, i0 = block * kBlock + lane * 4;
+    float p[8], g[8], m[8], q[8];
+    uint32_t cm[2], cs[2];
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+        const int64_t i = i0 + u * 128;
+        if (FULL) {
+            cm[u] = *(const uint32_t*)((const uint8_t*)e.m + i);
+            cs[u] = *(const uint32_t*)((const uint8_t*)e.v + i);
+            load4((const G*)e.g + i, g + 4 * u);
+            load4((const P*)e.p + i, p + 4 * u);
+        } else {
+            cm[u] = load4((const uint8_t*)e.m, i, n, vec);
+            cs[u] = load4((const uint8_t*)e.v, i, n, vec);
+            load4((const G*)e.g, i, n, vec, g + 4 * u);
+            load4((const P*)e.p, i, n, vec, p + 4 * u);
+        }
+    }
+    const float dm = power((int)e.m_exp[block] - 127), ds = power((int)e.v_exp[block] - 127);
+    uint32_t tm = 0, ts = 0;
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+        decode4(cm[u], dm, m + 4 * u);
+        decode4(cs[u], ds, q + 4 * u);
+#pragma unroll
+        for (int j = 4 * u; j < 4 * u + 4; j++) {
+            const float gj = __fmul_rn(g[j], s.scale);
+            m[j] = __fadd_rn(__fmul_rn(m[j], h.beta1), __fmul_rn(gj, h.rest1));
+            q[j] = __fsqrt_rn(__fadd_rn(__fmul_rn(__fmul_rn(q[j], q[j]), h.beta2),
+                                        __fmul_rn(__fmul_rn(gj, gj), h.rest2)));
+            p[j] = stepped(p[j], m[j], q[j], s);
+            tm = max(tm, __float_as_uint(m[j]) & 0x7fffffffu);
+            ts = max(ts, __float_as_uint(q[j]));
+        }
+    }
+    tm = __reduce_max_sync(0xffffffffu, tm);
+    ts = __reduce_max_sync(0xffffffffu, ts);
+    uint32_t nm = exponent_of(tm), ns = exponent_of(ts);
+    const uint32_t hash = key + (uint32_t)(i0 >> 32) * 0xBB67AE85u + (uint32_t)i0 * 0x9E3779B1u;
+    uint32_t wm[2], ws[2];
+    // 2^(127 - exponent + kCodeScale) has to be a number: exponents to 156, moments under 2^37
+    if (max(tm, ts) < 0x7f800000u && max(nm, ns) <= 156u) {
+        const float im = power(127 + kCodeScale - (int)nm), is = power(127 + kCodeScale - (int)ns);
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            uint32_t a[4], b[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint32_t bits = mix(hash + (uint32_t)(u * 128 + j) * 0x9E3779B1u);
+                const uint32_t x = __float_as_uint(m[4 * u + j] * im) + random_m(bits);   // the sign stays in bit 31
+                a[j] = x << 4 | (x & 0x80000000u);
+                b[j] = above_zero(__float_as_uint(q[4 * u + j] * is) + random_s(bits), q[4 * u + j]) << 4;
+            }
+            wm[u] = top_bytes(a);
+            ws[u] = top_bytes(b);
+        }
+    } else {
+        tm = ts = 0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            tm = max(tm, finite_bits(m[j]));
+            ts = max(ts, finite_bits(q[j]));
+        }
+        nm = exponent_of(__reduce_max_sync(0xffffffffu, tm));
+        ns = exponent_of(__reduce_max_sync(0xffffffffu, ts));
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            wm[u] = ws[u] = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint32_t bits = mix(hash + (uint32_t)(u * 128 + j) * 0x9E3779B1u);
+                wm[u] |= odd_code(m[4 * u + j], nm, random_m(bits), false) << (8 * j);
+                ws[u] |= odd_code(q[4 * u + j], ns, random_s(bits), true) << (8 * j);
+            }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+        const int64_t i = i0 + u * 128;
+        if (FULL) {
+            store4((P*)e.p + i, p + 4 * u);
+            *(uint32_t*)((uint8_t*)e.m + i) = wm[u];
+            *(uint32_t*)((uint8_t*)e.v + i) = ws[u];
+            if (e.copy) store4((bf16*)e.copy + i, p + 4 * u);
+        } else {
+            store4((P*)e.p, i, n, vec, p + 4 * u);
+            store4((uint8_t*)e.m, i, n, vec, wm[u]);
+            store4((uint8_t*)e.v, i, n, vec, ws[u]);
+            if (e.copy) store4((bf16*)e.copy, i, n, vec, p + 4 * u);
+        }
+    }
+    if (lane == 0) {
+        e.m_exp[block] = (uint8_t)nm;
+        e.v_exp[block] = (uint8_t)ns;
+    }
+}
+
 template <typename P, typename G, int CAP>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) adamw8_kernel(const __grid_constant__ Table<CAP> t) {
     const Step s = step_of(t.h);
-    const float b1 = t.h.beta1, b2 = t.h.beta2, r1 = t.h.rest1, r2 = t.h.rest2;
     const int64_t chunks = t.start[t.n];
-    const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    int k = find(t, blockIdx.x);
     for (int64_t c = blockIdx.x; c < chunks; c += gridDim.x) {
-        const int k = find(t, c);
+        k = advance(t, k, c);
         const Entry& e = t.e[k];
         const bool vec = t.vec[k];
-        const int64_t n = e.n, block = (c - t.start[k]) * (kChunk / kBlock) + warp, i0 = block * kBlock;
-        if (i0 >= n) continue;   // the whole warp
-        // lane l holds elements 4 l .. 4 l + 3 of both halves of the block
-        float p[8], g[8], m[8], q[8];
-        uint32_t cm[2], cs[2];
-        const uint32_t em = e.m_exp[block], es = e.v_exp[block];
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const int64_t i = i0 + u * 128 + lane * 4;
-            load4((const P*)e.p, i, n, vec, p + 4 * u);
-            load4((const G*)e.g, i, n, vec, g + 4 * u);
-            cm[u] = load4((const uint8_t*)e.m, i, n, vec);
-            cs[u] = load4((const uint8_t*)e.v, i, n, vec);
-        }
-        const float dm = power(em), ds = power(es);
-        uint32_t tm = 0, ts = 0;
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            decode4(cm[u], dm, m + 4 * u);
-            decode4(cs[u], ds, q + 4 * u);
-#pragma unroll
-            for (int j = 4 * u; j < 4 * u + 4; j++) {
-                const float gj = __fmul_rn(g[j], s.scale);
-                m[j] = __fadd_rn(__fmul_rn(m[j], b1), __fmul_rn(gj, r1));
-                q[j] = __fsqrt_rn(__fadd_rn(__fmul_rn(__fmul_rn(q[j], q[j]), b2), __fmul_rn(__fmul_rn(gj, gj), r2)));
-                p[j] = stepped(p[j], m[j], q[j], s);
-                tm = max(tm, magnitude(m[j]));
-                ts = max(ts, magnitude(q[j]));
-            }
-        }
-        const uint32_t nm = exponent_of(__reduce_max_sync(0xffffffffu, tm));
-        const uint32_t ns = exponent_of(__reduce_max_sync(0xffffffffu, ts));
-        const float im = power(254u - nm), is = power(254u - ns);
-        const uint32_t key = mix(s.key ^ (t.h.first + k)) + (uint32_t)(i0 >> 32) * 0xBB67AE85u;
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const int64_t i = i0 + u * 128 + lane * 4;
-            uint32_t wm = 0, ws = 0;
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const float a = m[4 * u + j], b = q[4 * u + j];
-                const uint32_t bits = mix(key + ((uint32_t)i + j) * 0x9E3779B1u);
-                uint32_t x = encode(fabsf(a) * im, (bits & 0xffffu) << 4 | 8u);
-                if (x) x |= a < 0.f ? 0x80u : 0u;
-                if (!isfinite(a)) x = 0x7fu;
-                uint32_t y = encode(b * is, (bits >> 16) << 4 | 8u);
-                if (b > 0.f && !y) y = 1u;
-                if (!isfinite(b)) y = 0x7fu;
-                wm |= x << (8 * j);
-                ws |= y << (8 * j);
-            }
-            if (i < n) {
-                store4((P*)e.p, i, n, vec, p + 4 * u);
-                store4((uint8_t*)e.m, i, n, vec, wm);
-                store4((uint8_t*)e.v, i, n, vec, ws);
-                if (e.copy) store4((bf16*)e.copy, i, n, vec, p + 4 * u);
-            }
-        }
-        if (lane == 0) {
-            e.m_exp[block] = (uint8_t)nm;
-            e.v_exp[block] = (uint8_t)ns;
-        }
+        const int64_t block = (c - t.start[k]) * (kChunk / kBlock) + threadIdx.x / 32;
+        const uint32_t key = mix(s.key ^ (t.h.first + k));
+        if (vec && (block + 1) * kBlock <= e.n) adamw8_block<P, G, true>(e, block, true, t.h, s, key);
+        else if (block * kBlock < e.n) adamw8_block<P, G, false>(e, block, vec, t.h, s, key);
     }
 }
 
 // -------------------------------------------------------------- grad norm --
-// part[blockIdx.x] = the CTA's sum of squares: f32 over a chunk's 8 elements a
-// thread, f64 over the chunks.
+__device__ __forceinline__ float sumsq16(const uint4 a, const float*) {
+    const float x = __uint_as_float(a.x), y = __uint_as_float(a.y), z = __uint_as_float(a.z), w = __uint_as_float(a.w);
+    return (x * x + y * y) + (z * z + w * w);
+}
+__device__ __forceinline__ float sumsq16(const uint4 a, const bf16*) {
+    const float x = bf16_lo(a.x) * bf16_lo(a.x) + bf16_hi(a.x) * bf16_hi(a.x);
+    const float y = bf16_lo(a.y) * bf16_lo(a.y) + bf16_hi(a.y) * bf16_hi(a.y);
+    const float z = bf16_lo(a.z) * bf16_lo(a.z) + bf16_hi(a.z) * bf16_hi(a.z);
+    const float w = bf16_lo(a.w) * bf16_lo(a.w) + bf16_hi(a.w) * bf16_hi(a.w);
+    return (x + y) + (z + w);
+}
+
+// part[blockIdx.x] = the CTA's sum of squares: f32 over a chunk's 32 elements a
+// thread, f64 over the chunks.  All of a chunk's loads are in flight at once.
 template <typename G, int CAP>
 __global__ void __launch_bounds__(kThreads) sumsq_kernel(const __grid_constant__ Table<CAP> t, double* __restrict__ part) {
+    constexpr int V = 16 / sizeof(G), L = kNormChunk / kThreads / V;
     __shared__ double red[kThreads / 32];
     const int64_t chunks = t.start[t.n];
     double acc = 0.0;
+    int k = find(t, blockIdx.x);
     for (int64_t c = blockIdx.x; c < chunks; c += gridDim.x) {
-        const int k = find(t, c);
-        const bool vec = t.vec[k];
-        const int64_t n = t.e[k].n, i0 = (c - t.start[k]) * kChunk + threadIdx.x * 4;
+        k = advance(t, k, c);
+        const G* g = (const G*)t.e[k].g;
+        const int64_t i0 = (c - t.start[k]) * kNormChunk, n = t.e[k].n;
         float s = 0.f;
+        if (t.vec[k] && i0 + kNormChunk <= n) {
+            uint4 a[L];
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const int64_t i = i0 + u * (kChunk / 2);
-            if (i >= n) continue;
-            float g[4];
-            load4((const G*)t.e[k].g, i, n, vec, g);
+            for (int u = 0; u < L; u++) a[u] = *reinterpret_cast<const uint4*>(g + i0 + (u * kThreads + threadIdx.x) * V);
 #pragma unroll
-            for (int j = 0; j < 4; j++) s += g[j] * g[j];
+            for (int u = 0; u < L; u++) s += sumsq16(a[u], g);
+        } else {
+#pragma unroll 8
+            for (int64_t i = i0 + threadIdx.x; i < n && i < i0 + kNormChunk; i += kThreads) {
+                const float x = load1(g + i);
+                s += x * x;
+            }
         }
         acc += s;
     }
@@ -386,17 +476,17 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const double* __restrict
 }
 
 // ------------------------------------------------------------------- host --
-int64_t chunks_of(int64_t n) { return (n + kChunk - 1) / kChunk; }
+int64_t chunks_of(int64_t n, int chunk) { return (n + chunk - 1) / chunk; }
 
-// Fills a table with tensors [at, at + count) of a list; returns its chunks.
+// Fills a table with the first tensors of a list; returns its chunks.
 template <int CAP>
-int64_t fill(Table<CAP>& t, const Entry* e, const uint8_t* vec, int count) {
+int64_t fill(Table<CAP>& t, const Entry* e, const uint8_t* vec, int count, int chunk) {
     t.n = count;
     t.start[0] = 0;
     for (int k = 0; k < count; k++) {
         t.e[k] = e[k];
         t.vec[k] = vec[k];
-        t.start[k + 1] = t.start[k] + chunks_of(e[k].n);
+        t.start[k + 1] = t.start[k] + chunks_of(e[k].n, chunk);
     }
     return t.start[count];
 }
@@ -411,7 +501,7 @@ bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) &
 template <typename P, typename G, int CAP>
 int adamw_launch(tb_ctx* ctx, int bits, const Entry* e, const uint8_t* vec, int count, const Hyper& h) {
     Table<CAP> t;
-    const int64_t chunks = fill(t, e, vec, count);
+    const int64_t chunks = fill(t, e, vec, count, kChunk);
     if (!chunks) return TB_OK;
     t.h = h;
     return launch(ctx, bits == 8 ? "adamw8" : "adamw", bits == 8 ? adamw8_kernel<P, G, CAP> : adamw_kernel<P, G, CAP>,
@@ -421,7 +511,7 @@ int adamw_launch(tb_ctx* ctx, int bits, const Entry* e, const uint8_t* vec, int 
 template <typename G, int CAP>
 int sumsq_launch(tb_ctx* ctx, const Entry* e, const uint8_t* vec, int count, double* part) {
     Table<CAP> t;
-    const int64_t chunks = fill(t, e, vec, count);
+    const int64_t chunks = fill(t, e, vec, count, kNormChunk);
     t.h = Hyper{};
     // every launch writes its own row of partial sums, of one CTA where there is nothing to add
     return launch(ctx, "grad_norm", sumsq_kernel<G, CAP>, dim3(chunks ? grid_for(ctx, chunks) : 1u), dim3(kThreads), 0, t,
@@ -619,8 +709,8 @@ int tb_grad_norm(tb_ctx* ctx, int dtype, const void* const* grads, const int64_t
             e[k] = Entry{};
             e[k].g = grads[at + k];
             e[k].n = sizes[at + k];
-            vec[k] = aligned(e[k].g, 4 * es);
-            chunks += chunks_of(e[k].n);
+            vec[k] = aligned16(e[k].g);
+            chunks += chunks_of(e[k].n, kNormChunk);
         }
         auto go = [&](auto small, auto large) {
             return cap == kSmallTable ? small(ctx, e, vec, count, part + parts) : large(ctx, e, vec, count, part + parts);

@@ -90,7 +90,7 @@ def encode(x, u, root):
     code = ((z.view(np.uint32).astype(np.int64) + ((u.astype(np.int64) << 4) | 8)) >> 20) - np.where(low, 968, 960)
     if root:
         code = np.where((size > 0) & (code == 0), 1, code)
-    code = np.where((x < 0) & (code > 0), code | 0x80, code)
+    code = np.where(np.signbit(x) & (not root), code | 0x80, code)
     code = np.where(fine, code, 0x7F)
     return code.astype(np.uint8).reshape(-1)[:n], e.astype(np.uint8)
 

@@ -356,13 +356,13 @@ def test_grad_norm(dtype, sizes):
     g = [rounded(r.standard_normal(n) * 10.0 ** r.uniform(-3, 1), dtype) for n in sizes]
     ts = [place(a, dtype, odd=k % 2 == 1)[0] for k, a in enumerate(g)]
     want = np.sqrt(sum(float((a.astype(np.float64) ** 2).sum()) for a in g))
-    # squares and 8 additions in f32: 9 half steps of the sum, half of that of the root, and its own rounding
+    # squares and 32 additions in f32: 33 half steps of the sum, half of that of the root, and its own rounding
     norm = o.grad_norm(ts)
-    assert abs(float(norm) - want) <= 6 * u.U32 * want
+    assert abs(float(norm) - want) <= 18 * u.U32 * want
     for top in (want / 3, want * 3, 0.0):
         norm2, scale = o.grad_norm(ts, max_norm=top)
         assert torch.equal(norm, norm2)
-        assert abs(float(scale) - min(1.0, top / (want + 1e-6))) <= 8 * u.U32
+        assert abs(float(scale) - min(1.0, top / (want + 1e-6))) <= 20 * u.U32
 
 
 def test_grad_norm_of_nothing_and_of_what_is_not_finite():
@@ -415,7 +415,7 @@ def test_offsets_past_32_bits():
     p[-k:], g[-k:] = torch.from_numpy(hp).cuda(), torch.from_numpy(hg).cuda()
     norm = o.grad_norm([g])
     want = np.sqrt((hg.astype(np.float64) ** 2).sum())
-    assert abs(float(norm) - want) <= 6 * u.U32 * want
+    assert abs(float(norm) - want) <= 18 * u.U32 * want
     opt = o.AdamW([p], [g], lr=LR, betas=(B1, B2), eps=EPS, weight_decay=WD, state_bits=8, seed=3)
     opt.step()
     ref = o.AdamW([torch.from_numpy(hp).cuda().bfloat16()], [g[-k:].clone()], lr=LR, betas=(B1, B2), eps=EPS,
