@@ -22,7 +22,8 @@
 //    probability of the rest, by 16 bits each of a hash of (seed, step, tensor,
 //    element): the mean over the steps is the 32-bit moment's, and a run repeats.
 //  * Each operation up to the code is rounded by itself (no fused multiply-add),
-//    so the codes are defined bit for bit by the formula.
+//    so the codes are defined bit for bit by the formula, but for the last place
+//    of the square root.
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <math.h>
@@ -244,17 +245,17 @@ __device__ __forceinline__ float power(int e) {
     return __uint_as_float(e >= -126 ? (uint32_t)(e + 127) << 23 : 1u << (e + 149));
 }
 
-__device__ __forceinline__ void decode4(uint32_t w, float scale, float* v) {
+__device__ __forceinline__ void decode4(uint32_t w, float* v) {
     const __half2 a(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3));
     const __half2 b(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3));
     const float2 x = __half22float2(a), y = __half22float2(b);
-    v[0] = x.x * scale; v[1] = x.y * scale; v[2] = y.x * scale; v[3] = y.y * scale;
+    v[0] = x.x; v[1] = x.y; v[2] = y.x; v[3] = y.y;
 }
 
-__device__ __forceinline__ uint32_t exponent_of(uint32_t top) {
-    const uint32_t e = top >> 23;
-    return e > 7u ? e - 7u : 0u;
-}
+// The block's exponent for its largest value 2^e (1 + f).
+__device__ __forceinline__ int block_exponent(int e) { return max(e + 120, 0); }
+// floor(log2) of a float's bits, subnormal ones among them; for zero less than any exponent, and its half too.
+__device__ __forceinline__ int log2_of(uint32_t u) { return u >> 23 ? (int)(u >> 23) - 127 : u ? -118 - __clz(u) : -300; }
 
 // Codes.  x is scaled to put the code's smallest normal value, 2^-6, on f32's, 2^-126: then
 // the code is the f32's bits 20 to 26, in the subnormal range too, and what lies below them
@@ -272,11 +273,16 @@ __device__ __forceinline__ uint32_t top_bytes(const uint32_t* t) {
     return __byte_perm(__byte_perm(t[0], t[1], 0x0073), __byte_perm(t[2], t[3], 0x7300), 0x7610);
 }
 
-// A block with a value that is not finite (it becomes NaN, and does not count for the block's
-// exponent) or with an exponent too large for one factor: the scaling in two.
-__device__ __noinline__ uint32_t odd_code(float x, uint32_t e, uint32_t r, bool root) {
+__device__ __forceinline__ float sqrt_fast(float x) {
+    float y;
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// The code of a value of any kind: what is not finite becomes NaN; the scaling in two steps.
+__device__ __forceinline__ uint32_t any_code(float x, int e, uint32_t r, bool root) {
     if (!isfinite(x)) return 0x7fu;
-    uint32_t t = __float_as_uint(fabsf(x) * power(127 - (int)e) * power(kCodeScale)) + r;
+    uint32_t t = __float_as_uint(fabsf(x) * power(127 - e) * power(kCodeScale)) + r;
     if (root) t = above_zero(t, x);
     return t >> 20 | (root ? 0u : __float_as_uint(x) >> 24 & 0x80u);
 }
@@ -285,107 +291,132 @@ __device__ __forceinline__ uint32_t finite_bits(float x) {
     return u < 0x7f800000u ? u : 0u;
 }
 
-// One block of 256 elements from i0 of tensor e, by a warp: lane l has elements 4 l .. 4 l + 3
-// of both halves.  FULL: all of them exist, and their addresses allow vectors.
-template <typename P, typename G, bool FULL>
-__device__ __forceinline__ void adamw8_block(const Entry& e, int64_t block, bool vec, const Hyper& h, const Step& s,
-                                             uint32_t key) {
-    const int lane = threadIdx.x & 31;
-    const int64_t n = e.n, i0 = block * kBlock + lane * 4;
-    float p[8], g[8], m[8], q[8];
+// Where a lane's element k lies in its block: lane l has 4 l .. 4 l + 3 of both halves.
+__device__ __forceinline__ int64_t place(int64_t block, int u) { return block * kBlock + u * 128 + (threadIdx.x & 31) * 4; }
+
+__device__ __forceinline__ uint32_t hash_of(uint32_t key, int64_t i) {
+    return key + (uint32_t)(i >> 32) * 0xBB67AE85u + (uint32_t)i * 0x9E3779B1u;
+}
+
+// One block of 256 elements, by a warp, every operation by itself: for blocks at the ends of
+// tensors and at the ends of the range.
+template <typename P, typename G>
+__device__ __noinline__ void adamw8_odd_block(const Entry& e, int64_t block, bool vec, const Hyper& h, const Step& s,
+                                              uint32_t key) {
+    const int64_t n = e.n;
+    float p[8], g[8], m[8], v[8];
+    const float dm = power((int)e.m_exp[block] - 127), ds = power((int)e.v_exp[block] - 127);
+    uint32_t tm = 0, tv = 0;
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+        const int64_t i = place(block, u);
+        decode4(load4((const uint8_t*)e.m, i, n, vec), m + 4 * u);
+        decode4(load4((const uint8_t*)e.v, i, n, vec), v + 4 * u);
+        load4((const G*)e.g, i, n, vec, g + 4 * u);
+        load4((const P*)e.p, i, n, vec, p + 4 * u);
+#pragma unroll
+        for (int j = 4 * u; j < 4 * u + 4; j++) {
+            const float gj = __fmul_rn(g[j], s.scale), sj = v[j] * ds;
+            m[j] = __fadd_rn(__fmul_rn(m[j] * dm, h.beta1), __fmul_rn(gj, h.rest1));
+            v[j] = __fsqrt_rn(__fadd_rn(__fmul_rn(__fmul_rn(sj, sj), h.beta2), __fmul_rn(__fmul_rn(gj, gj), h.rest2)));
+            p[j] = stepped(p[j], m[j], v[j], s);
+            tm = max(tm, finite_bits(m[j]));
+            tv = max(tv, finite_bits(v[j]));
+        }
+    }
+    const int nm = block_exponent(log2_of(__reduce_max_sync(0xffffffffu, tm)));
+    const int ns = block_exponent(log2_of(__reduce_max_sync(0xffffffffu, tv)));
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+        const int64_t i = place(block, u);
+        uint32_t wm = 0, ws = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint32_t bits = mix(hash_of(key, i) + (uint32_t)j * 0x9E3779B1u);
+            wm |= any_code(m[4 * u + j], nm, random_m(bits), false) << (8 * j);
+            ws |= any_code(v[4 * u + j], ns, random_s(bits), true) << (8 * j);
+        }
+        store4((P*)e.p, i, n, vec, p + 4 * u);
+        store4((uint8_t*)e.m, i, n, vec, wm);
+        store4((uint8_t*)e.v, i, n, vec, ws);
+        if (e.copy) store4((bf16*)e.copy, i, n, vec, p + 4 * u);
+    }
+    if ((threadIdx.x & 31) == 0) {
+        e.m_exp[block] = (uint8_t)nm;
+        e.v_exp[block] = (uint8_t)ns;
+    }
+}
+
+// A whole block at aligned addresses; false, with nothing written, where it is not a common
+// one.  The common case folds the exponents into the betas (exact, as they are powers of two)
+// and takes the hardware's square root (2^-23), which flushes what is under 2^-126.
+template <typename P, typename G>
+__device__ __forceinline__ bool adamw8_block(const Entry& e, int64_t block, const Hyper& h, const Step& s, uint32_t key) {
+    const int64_t i0 = place(block, 0);
+    float p[8], g[8], m[8], v[8];
     uint32_t cm[2], cs[2];
 #pragma unroll
     for (int u = 0; u < 2; u++) {
         const int64_t i = i0 + u * 128;
-        if (FULL) {
-            cm[u] = *(const uint32_t*)((const uint8_t*)e.m + i);
-            cs[u] = *(const uint32_t*)((const uint8_t*)e.v + i);
-            load4((const G*)e.g + i, g + 4 * u);
-            load4((const P*)e.p + i, p + 4 * u);
-        } else {
-            cm[u] = load4((const uint8_t*)e.m, i, n, vec);
-            cs[u] = load4((const uint8_t*)e.v, i, n, vec);
-            load4((const G*)e.g, i, n, vec, g + 4 * u);
-            load4((const P*)e.p, i, n, vec, p + 4 * u);
-        }
+        cm[u] = *(const uint32_t*)((const uint8_t*)e.m + i);
+        cs[u] = *(const uint32_t*)((const uint8_t*)e.v + i);
+        load4((const G*)e.g + i, g + 4 * u);
+        load4((const P*)e.p + i, p + 4 * u);
     }
-    const float dm = power((int)e.m_exp[block] - 127), ds = power((int)e.v_exp[block] - 127);
-    uint32_t tm = 0, ts = 0;
+    const int em = e.m_exp[block], es = e.v_exp[block];
+    // m beta1 = code * bm and s^2 beta2 = code^2 * bs
+    const float ds = power(es - 127), bm = power(em - 127) * h.beta1, bs = ds * ds * h.beta2;
+    uint32_t tm = 0, tv = 0;
 #pragma unroll
     for (int u = 0; u < 2; u++) {
-        decode4(cm[u], dm, m + 4 * u);
-        decode4(cs[u], ds, q + 4 * u);
+        decode4(cm[u], m + 4 * u);
+        decode4(cs[u], v + 4 * u);
 #pragma unroll
         for (int j = 4 * u; j < 4 * u + 4; j++) {
             const float gj = __fmul_rn(g[j], s.scale);
-            m[j] = __fadd_rn(__fmul_rn(m[j], h.beta1), __fmul_rn(gj, h.rest1));
-            q[j] = __fsqrt_rn(__fadd_rn(__fmul_rn(__fmul_rn(q[j], q[j]), h.beta2),
-                                        __fmul_rn(__fmul_rn(gj, gj), h.rest2)));
-            p[j] = stepped(p[j], m[j], q[j], s);
+            m[j] = __fadd_rn(__fmul_rn(m[j], bm), __fmul_rn(gj, h.rest1));
+            v[j] = __fadd_rn(__fmul_rn(__fmul_rn(v[j], v[j]), bs), __fmul_rn(__fmul_rn(gj, gj), h.rest2));
             tm = max(tm, __float_as_uint(m[j]) & 0x7fffffffu);
-            ts = max(ts, __float_as_uint(q[j]));
+            tv = max(tv, __float_as_uint(v[j]));
         }
     }
     tm = __reduce_max_sync(0xffffffffu, tm);
-    ts = __reduce_max_sync(0xffffffffu, ts);
-    uint32_t nm = exponent_of(tm), ns = exponent_of(ts);
-    const uint32_t hash = key + (uint32_t)(i0 >> 32) * 0xBB67AE85u + (uint32_t)i0 * 0x9E3779B1u;
-    uint32_t wm[2], ws[2];
-    // 2^(127 - exponent + kCodeScale) has to be a number: exponents to 156, moments under 2^37
-    if (max(tm, ts) < 0x7f800000u && max(nm, ns) <= 156u) {
-        const float im = power(127 + kCodeScale - (int)nm), is = power(127 + kCodeScale - (int)ns);
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            uint32_t a[4], b[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const uint32_t bits = mix(hash + (uint32_t)(u * 128 + j) * 0x9E3779B1u);
-                const uint32_t x = __float_as_uint(m[4 * u + j] * im) + random_m(bits);   // the sign stays in bit 31
-                a[j] = x << 4 | (x & 0x80000000u);
-                b[j] = above_zero(__float_as_uint(q[4 * u + j] * is) + random_s(bits), q[4 * u + j]) << 4;
-            }
-            wm[u] = top_bytes(a);
-            ws[u] = top_bytes(b);
-        }
-    } else {
-        tm = ts = 0;
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            tm = max(tm, finite_bits(m[j]));
-            ts = max(ts, finite_bits(q[j]));
-        }
-        nm = exponent_of(__reduce_max_sync(0xffffffffu, tm));
-        ns = exponent_of(__reduce_max_sync(0xffffffffu, ts));
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            wm[u] = ws[u] = 0;
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const uint32_t bits = mix(hash + (uint32_t)(u * 128 + j) * 0x9E3779B1u);
-                wm[u] |= odd_code(m[4 * u + j], nm, random_m(bits), false) << (8 * j);
-                ws[u] |= odd_code(q[4 * u + j], ns, random_s(bits), true) << (8 * j);
-            }
-        }
-    }
+    tv = __reduce_max_sync(0xffffffffu, tv);
+    // Finite moments, under 2^37 (2^(127 - exponent + kCodeScale) has to be a number); held exponents whose
+    // products with a code are normal numbers, or codes that are all 0 (a new tensor's); a largest root above
+    // 2^-42, next to which a flushed one rounds as its own value does, or none; and an eps that a flushed root
+    // can do with.
+    const bool fresh = !(cm[0] | cm[1] | cs[0] | cs[1]);
+    if (!(tm < 164u << 23 && tv < 201u << 23 && ((em >= 32 && es >= 84) || __all_sync(0xffffffffu, fresh)) &&
+          (tv >= 43u << 23 || tv == 0) && s.eps > 1e-30f))
+        return false;
+    const int nm = block_exponent(log2_of(tm)), ns = block_exponent(log2_of(tv) >> 1);   // no root rounds up to a power of two
+    const float im = power(127 + kCodeScale - nm), is = power(127 + kCodeScale - ns);
+    const uint32_t hash = hash_of(key, i0);
 #pragma unroll
     for (int u = 0; u < 2; u++) {
         const int64_t i = i0 + u * 128;
-        if (FULL) {
-            store4((P*)e.p + i, p + 4 * u);
-            *(uint32_t*)((uint8_t*)e.m + i) = wm[u];
-            *(uint32_t*)((uint8_t*)e.v + i) = ws[u];
-            if (e.copy) store4((bf16*)e.copy + i, p + 4 * u);
-        } else {
-            store4((P*)e.p, i, n, vec, p + 4 * u);
-            store4((uint8_t*)e.m, i, n, vec, wm[u]);
-            store4((uint8_t*)e.v, i, n, vec, ws[u]);
-            if (e.copy) store4((bf16*)e.copy, i, n, vec, p + 4 * u);
+        uint32_t a[4], b[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int k = 4 * u + j;
+            const float root = sqrt_fast(v[k]);
+            p[k] = stepped(p[k], m[k], root, s);
+            const uint32_t bits = mix(hash + (uint32_t)(u * 128 + j) * 0x9E3779B1u);
+            const uint32_t x = __float_as_uint(m[k] * im) + random_m(bits);   // the sign stays in bit 31
+            a[j] = x << 4 | (x & 0x80000000u);
+            b[j] = above_zero(__float_as_uint(root * is) + random_s(bits), v[k]) << 4;
         }
+        store4((P*)e.p + i, p + 4 * u);
+        *(uint32_t*)((uint8_t*)e.m + i) = top_bytes(a);
+        *(uint32_t*)((uint8_t*)e.v + i) = top_bytes(b);
+        if (e.copy) store4((bf16*)e.copy + i, p + 4 * u);
     }
-    if (lane == 0) {
+    if ((threadIdx.x & 31) == 0) {
         e.m_exp[block] = (uint8_t)nm;
         e.v_exp[block] = (uint8_t)ns;
     }
+    return true;
 }
 
 template <typename P, typename G, int CAP>
@@ -399,8 +430,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) adamw8_kernel(const __gr
         const bool vec = t.vec[k];
         const int64_t block = (c - t.start[k]) * (kChunk / kBlock) + threadIdx.x / 32;
         const uint32_t key = mix(s.key ^ (t.h.first + k));
-        if (vec && (block + 1) * kBlock <= e.n) adamw8_block<P, G, true>(e, block, true, t.h, s, key);
-        else if (block * kBlock < e.n) adamw8_block<P, G, false>(e, block, vec, t.h, s, key);
+        if (block * kBlock >= e.n) continue;   // the whole warp
+        if (vec && (block + 1) * kBlock <= e.n && adamw8_block<P, G>(e, block, t.h, s, key)) continue;
+        adamw8_odd_block<P, G>(e, block, vec, t.h, s, key);
     }
 }
 

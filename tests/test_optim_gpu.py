@@ -91,6 +91,17 @@ class Model:
                     state=self.state, step_count=step_count)
         return ops().AdamW(self.params, self.grads, **{**args, **kw})
 
+    def check_codes(self, k, want):
+        """Holds the codes of tensor k to adamw8_moments'; the host takes them over."""
+        cm, em, cs, es, either = want
+        got = {name: ts[k].cpu().numpy() for name, ts in self.codes.items()}
+        np.testing.assert_array_equal(got["m"], cm, err_msg="m")
+        np.testing.assert_array_equal(got["m_exp"], em, err_msg="m_exp")
+        np.testing.assert_array_equal(got["s_exp"], es, err_msg="s_exp")
+        off = np.abs(got["s"].astype(int) - cs)
+        assert np.all((off == 0) | ((off == 1) & either)), "s"
+        self.m[k], self.s[k] = (cm, em), (got["s"], es)
+
     def check(self, t, scale=1.0, seed=0, lr=LR, b1=B1, b2=B2, eps=EPS, wd=WD):
         """Holds the device's tensors after step t to the host's; the host takes them over."""
         scale = float(np.float32(scale))
@@ -98,11 +109,8 @@ class Model:
             if self.bits == 32:
                 m, v = self.m[k], self.v[k]
             else:
-                cm, em, cs, es, m1, s1 = u.adamw8_moments(self.g[k], *self.m[k], *self.s[k], seed, t, k, b1, b2, scale)
                 m, v = u.held(*self.m[k]), u.held(*self.s[k]).astype(np.float64) ** 2
-                for name, want in (("m", cm), ("m_exp", em), ("s", cs), ("s_exp", es)):
-                    np.testing.assert_array_equal(self.codes[name][k].cpu().numpy(), want, err_msg=f"{name} of {n}")
-                self.m[k], self.s[k] = (cm, em), (cs, es)
+                self.check_codes(k, u.adamw8_moments(self.g[k], *self.m[k], *self.s[k], seed, t, k, b1, b2, scale))
             p, m1, v1, up, size, div = u.adamw64(self.p[k], self.g[k], m, v, t, lr, b1, b2, eps, wd, scale)
             bm, bp = u.bounds(self.p[k], up, size, div, p if self.pt == BF16 else None)
             got = host(self.params[k])
@@ -200,14 +208,34 @@ def test_adamw_8_bits_at_the_edges_of_the_range():
     o = m.optimiser()
     for t in (1, 2, 3):
         o.step()
-        cm, em, cs, es, m1, s1 = u.adamw8_moments(m.g[0], *m.m[0], *m.s[0], 0, t, 0, B1, B2, 1.0)
-        for name, want in (("m", cm), ("m_exp", em), ("s", cs), ("s_exp", es)):
-            np.testing.assert_array_equal(m.codes[name][0].cpu().numpy(), want, err_msg=f"{name} at {t}")
-        m.m[0], m.s[0] = (cm, em), (cs, es)
+        m.check_codes(0, u.adamw8_moments(m.g[0], *m.m[0], *m.s[0], 0, t, 0, B1, B2, 1.0))
         p = host(m.params[0]).reshape(12, 256)
         bad = ~np.isfinite(p)
         assert bad[10, :3].all() and not np.delete(bad, 10, 0).any() and not bad[10, 5:].any()
     assert (host(m.state["s"][0]).reshape(12, 256)[10, 5:] < 256).all()
+
+
+def test_adamw_8_bits_over_all_sizes():
+    """A block for each power of two of the gradient, and the sizes within a block spread over forty more."""
+    ops()
+    k = 2 * 230
+    m = Model([256 * k], F32, F32, False, 8, seed=16)
+    r = rng(2)
+    with np.errstate(under="ignore", over="ignore"):
+        g = r.standard_normal((k, 256)) * 2.0 ** (np.arange(k)[:, None] // 2 - 150)
+        g[1::2] *= 2.0 ** r.uniform(-40, 0, (k // 2, 256))
+        m.g[0] = g.astype(np.float32).reshape(-1)
+    m.grads[0].copy_(torch.from_numpy(m.g[0]))
+    for name in m.codes:
+        m.codes[name][0].zero_()
+    m.m, m.s = [(np.zeros(256 * k, np.uint8), np.zeros(k, np.uint8))], [(np.zeros(256 * k, np.uint8), np.zeros(k, np.uint8))]
+    o = m.optimiser(eps=1e-12)
+    for t in (1, 2, 3, 4):
+        o.step()
+        m.check_codes(0, u.adamw8_moments(m.g[0], *m.m[0], *m.s[0], 0, t, 0, B1, B2, 1.0))
+        if t == 2:   # a smaller gradient, so that the held moments count
+            m.g[0] = (m.g[0] * np.float32(0.01)).astype(np.float32)
+            m.grads[0].copy_(torch.from_numpy(m.g[0]))
 
 
 @pytest.mark.parametrize("bits", [32, 8])
