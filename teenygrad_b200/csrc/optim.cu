@@ -43,7 +43,7 @@ constexpr int kThreads = 256;
 constexpr int kChunk = 2048;      // elements of one tensor that a CTA takes at a time
 constexpr int kNormChunk = 8192;  // the same of the gradient norm
 constexpr int kBlock = 256;       // elements that share an exponent: one warp, 8 a lane
-constexpr int kCtasPerSm = 4;
+constexpr int kCtasPerSm = 4, kCtasPerSm8 = 2;
 
 // Tensors a launch's parameters hold: 4 KB of them cost a launch nothing, 32 KB
 // some microseconds, so models of few tensors take the small table.
@@ -166,12 +166,15 @@ struct Step {
     uint32_t key;
 };
 
-__device__ __forceinline__ uint32_t mix(uint32_t x) {
-    // xor-shifts and odd multipliers (the fractions of sqrt 2 and sqrt 3), each a bijection
+// Xor-shifts and odd multipliers (the fractions of sqrt 2 and sqrt 3), each a bijection.
+__device__ __forceinline__ uint32_t mix_most(uint32_t x) {
     x ^= x >> 16;
     x *= 0x6A09E667u;
     x ^= x >> 15;
-    x *= 0xBB67AE85u;
+    return x * 0xBB67AE85u;
+}
+__device__ __forceinline__ uint32_t mix(uint32_t x) {
+    x = mix_most(x);
     return x ^ (x >> 16);
 }
 
@@ -239,6 +242,51 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) adamw_kernel(const __gri
     }
 }
 
+// Two f32 in one instruction, each rounded as by itself.
+struct F2 {
+    unsigned long long v;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void get(F2 a, float* v) { asm("mov.b64 {%0, %1}, %2;" : "=f"(v[0]), "=f"(v[1]) : "l"(a.v)); }
+__device__ __forceinline__ F2 mul(F2 a, F2 b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 fma(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+// Two sums.  Packed, they were contracted with the products they add; scalar ones with a rounding of their own are not.
+__device__ __forceinline__ void sums(F2 a, F2 b, float* v) {
+    float x[2], y[2];
+    get(a, x);
+    get(b, y);
+    v[0] = __fadd_rn(x[0], y[0]);
+    v[1] = __fadd_rn(x[1], y[1]);
+}
+// The largest of three sizes; NaN where one is NaN.
+__device__ __forceinline__ float largest(float a, float b, float c) {
+    float r;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float sqrt_fast(float x) {
+    float y;
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // ------------------------------------------------------------ 8-bit codes --
 // 2^e for e in [-149, 127], exact.
 __device__ __forceinline__ float power(int e) {
@@ -262,28 +310,24 @@ __device__ __forceinline__ int log2_of(uint32_t u) { return u >> 23 ? (int)(u >>
 // carries into it with probability rest / 2^20 when 16 random bits (and a half) are added.
 constexpr int kCodeScale = -120;
 
-__device__ __forceinline__ uint32_t random_m(uint32_t bits) { return (bits << 4 & 0xffff0u) + 8u; }
-__device__ __forceinline__ uint32_t random_s(uint32_t bits) { return (bits >> 12 & 0xffff0u) + 8u; }
-
-// What is above zero keeps a code above zero.
-__device__ __forceinline__ uint32_t above_zero(uint32_t t, float x) { return x > 0.f ? max(t, 1u << 20) : t; }
+// 16 random bits and a half each, from bit 8 on: with bits = mix(x), rm = (bits & 0xffff) << 8 | 0x80 and
+// rs = bits >> 16 << 8 | 0x80.  mix's last step only changes the low half, by the high one.
+__device__ __forceinline__ void random_bits(uint32_t x, uint32_t& rm, uint32_t& rs) {
+    x = mix_most(x);
+    rs = __byte_perm(x, 0x80u, 0x5324);
+    rm = __byte_perm(x, 0u, 0x4104) ^ rs;
+}
 
 // Bytes 3 of four words.
 __device__ __forceinline__ uint32_t top_bytes(const uint32_t* t) {
     return __byte_perm(__byte_perm(t[0], t[1], 0x0073), __byte_perm(t[2], t[3], 0x7300), 0x7610);
 }
 
-__device__ __forceinline__ float sqrt_fast(float x) {
-    float y;
-    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // The code of a value of any kind: what is not finite becomes NaN; the scaling in two steps.
 __device__ __forceinline__ uint32_t any_code(float x, int e, uint32_t r, bool root) {
     if (!isfinite(x)) return 0x7fu;
     uint32_t t = __float_as_uint(fabsf(x) * power(127 - e) * power(kCodeScale)) + r;
-    if (root) t = above_zero(t, x);
+    if (root && x > 0.f) t = max(t, 1u << 20);   // what is above zero keeps a code above zero
     return t >> 20 | (root ? 0u : __float_as_uint(x) >> 24 & 0x80u);
 }
 __device__ __forceinline__ uint32_t finite_bits(float x) {
@@ -332,9 +376,10 @@ __device__ __noinline__ void adamw8_odd_block(const Entry& e, int64_t block, boo
         uint32_t wm = 0, ws = 0;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const uint32_t bits = mix(hash_of(key, i) + (uint32_t)j * 0x9E3779B1u);
-            wm |= any_code(m[4 * u + j], nm, random_m(bits), false) << (8 * j);
-            ws |= any_code(v[4 * u + j], ns, random_s(bits), true) << (8 * j);
+            uint32_t rm, rs;
+            random_bits(hash_of(key, i) + (uint32_t)j * 0x9E3779B1u, rm, rs);
+            wm |= any_code(m[4 * u + j], nm, rm >> 4, false) << (8 * j);
+            ws |= any_code(v[4 * u + j], ns, rs >> 4, true) << (8 * j);
         }
         store4((P*)e.p, i, n, vec, p + 4 * u);
         store4((uint8_t*)e.m, i, n, vec, wm);
@@ -347,70 +392,119 @@ __device__ __noinline__ void adamw8_odd_block(const Entry& e, int64_t block, boo
     }
 }
 
+// Four values as they lie in memory.
+template <typename T>
+struct Raw4;
+template <>
+struct Raw4<float> {
+    float4 a;
+    __device__ __forceinline__ void load(const float* p) { a = *reinterpret_cast<const float4*>(p); }
+    __device__ __forceinline__ void get(float* v) const { v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; }
+};
+template <>
+struct Raw4<bf16> {
+    uint2 a;
+    __device__ __forceinline__ void load(const bf16* p) { a = *reinterpret_cast<const uint2*>(p); }
+    __device__ __forceinline__ void get(float* v) const {
+        v[0] = bf16_lo(a.x); v[1] = bf16_hi(a.x); v[2] = bf16_lo(a.y); v[3] = bf16_hi(a.y);
+    }
+};
+
+// What a step reads of a block.
+template <typename P, typename G>
+struct BlockIn {
+    Raw4<P> p[2];
+    Raw4<G> g[2];
+    uint32_t cm[2], cs[2];
+    uint8_t em, es;
+    __device__ __forceinline__ void load(const Entry& e, int64_t block) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int64_t i = place(block, u);
+            p[u].load((const P*)e.p + i);
+            g[u].load((const G*)e.g + i);
+            cm[u] = *(const uint32_t*)((const uint8_t*)e.m + i);
+            cs[u] = *(const uint32_t*)((const uint8_t*)e.v + i);
+        }
+        em = e.m_exp[block];
+        es = e.v_exp[block];
+    }
+};
+
 // A whole block at aligned addresses; false, with nothing written, where it is not a common
 // one.  The common case folds the exponents into the betas (exact, as they are powers of two)
 // and takes the hardware's square root (2^-23), which flushes what is under 2^-126.
 template <typename P, typename G>
-__device__ __forceinline__ bool adamw8_block(const Entry& e, int64_t block, const Hyper& h, const Step& s, uint32_t key) {
+__device__ __forceinline__ bool adamw8_block(const BlockIn<P, G>& in, const Entry& e, int64_t block, const Hyper& h,
+                                             const Step& s, uint32_t key) {
     const int64_t i0 = place(block, 0);
-    float p[8], g[8], m[8], v[8];
-    uint32_t cm[2], cs[2];
-#pragma unroll
-    for (int u = 0; u < 2; u++) {
-        const int64_t i = i0 + u * 128;
-        cm[u] = *(const uint32_t*)((const uint8_t*)e.m + i);
-        cs[u] = *(const uint32_t*)((const uint8_t*)e.v + i);
-        load4((const G*)e.g + i, g + 4 * u);
-        load4((const P*)e.p + i, p + 4 * u);
-    }
-    const int em = e.m_exp[block], es = e.v_exp[block];
+    const int em = in.em, es = in.es;
     // m beta1 = code * bm and s^2 beta2 = code^2 * bs
     const float ds = power(es - 127), bm = power(em - 127) * h.beta1, bs = ds * ds * h.beta2;
-    uint32_t tm = 0, tv = 0;
+    const F2 bm2 = f2(bm, bm), bs2 = f2(bs, bs), scale2 = f2(s.scale, s.scale), r1 = f2(h.rest1, h.rest1),
+             r2 = f2(h.rest2, h.rest2);
+    float m[8], v[8];
+    float top_m = 0.f, top_v = 0.f;
 #pragma unroll
     for (int u = 0; u < 2; u++) {
-        decode4(cm[u], m + 4 * u);
-        decode4(cs[u], v + 4 * u);
+        float g[4];
+        decode4(in.cm[u], m + 4 * u);
+        decode4(in.cs[u], v + 4 * u);
+        in.g[u].get(g);
 #pragma unroll
-        for (int j = 4 * u; j < 4 * u + 4; j++) {
-            const float gj = __fmul_rn(g[j], s.scale);
-            m[j] = __fadd_rn(__fmul_rn(m[j], bm), __fmul_rn(gj, h.rest1));
-            v[j] = __fadd_rn(__fmul_rn(__fmul_rn(v[j], v[j]), bs), __fmul_rn(__fmul_rn(gj, gj), h.rest2));
-            tm = max(tm, __float_as_uint(m[j]) & 0x7fffffffu);
-            tv = max(tv, __float_as_uint(v[j]));
+        for (int j = 0; j < 4; j += 2) {
+            const int k = 4 * u + j;
+            const F2 g2 = mul(f2(g[j], g[j + 1]), scale2), c2 = f2(v[k], v[k + 1]);
+            sums(mul(f2(m[k], m[k + 1]), bm2), mul(g2, r1), m + k);
+            sums(mul(mul(c2, c2), bs2), mul(mul(g2, g2), r2), v + k);
+            top_m = largest(top_m, m[k], m[k + 1]);
+            top_v = largest(top_v, v[k], v[k + 1]);
         }
     }
-    tm = __reduce_max_sync(0xffffffffu, tm);
-    tv = __reduce_max_sync(0xffffffffu, tv);
+    const uint32_t tm = __reduce_max_sync(0xffffffffu, __float_as_uint(top_m));
+    const uint32_t tv = __reduce_max_sync(0xffffffffu, __float_as_uint(top_v));
     // Finite moments, under 2^37 (2^(127 - exponent + kCodeScale) has to be a number); held exponents whose
     // products with a code are normal numbers, or codes that are all 0 (a new tensor's); a largest root above
     // 2^-42, next to which a flushed one rounds as its own value does, or none; and an eps that a flushed root
     // can do with.
-    const bool fresh = !(cm[0] | cm[1] | cs[0] | cs[1]);
+    const bool fresh = !(in.cm[0] | in.cm[1] | in.cs[0] | in.cs[1]);
     if (!(tm < 164u << 23 && tv < 201u << 23 && ((em >= 32 && es >= 84) || __all_sync(0xffffffffu, fresh)) &&
           (tv >= 43u << 23 || tv == 0) && s.eps > 1e-30f))
         return false;
     const int nm = block_exponent(log2_of(tm)), ns = block_exponent(log2_of(tv) >> 1);   // no root rounds up to a power of two
     const float im = power(127 + kCodeScale - nm), is = power(127 + kCodeScale - ns);
+    const F2 im2 = f2(im, im), is2 = f2(is, is), root2 = f2(s.root, s.root), eps2 = f2(s.eps, s.eps),
+             rate2 = f2(-s.rate, -s.rate), keep2 = f2(s.keep, s.keep);
     const uint32_t hash = hash_of(key, i0);
 #pragma unroll
     for (int u = 0; u < 2; u++) {
         const int64_t i = i0 + u * 128;
+        float p[4];
         uint32_t a[4], b[4];
+        in.p[u].get(p);
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
+        for (int j = 0; j < 4; j += 2) {
             const int k = 4 * u + j;
-            const float root = sqrt_fast(v[k]);
-            p[k] = stepped(p[k], m[k], root, s);
-            const uint32_t bits = mix(hash + (uint32_t)(u * 128 + j) * 0x9E3779B1u);
-            const uint32_t x = __float_as_uint(m[k] * im) + random_m(bits);   // the sign stays in bit 31
-            a[j] = x << 4 | (x & 0x80000000u);
-            b[j] = above_zero(__float_as_uint(root * is) + random_s(bits), v[k]) << 4;
+            const F2 m2 = f2(m[k], m[k + 1]), q2 = f2(sqrt_fast(v[k]), sqrt_fast(v[k + 1]));
+            float d[2], x[2], y[2];
+            get(fma(q2, root2, eps2), d);
+            get(fma(f2(p[j], p[j + 1]), keep2, mul(mul(m2, rate2), f2(rcp_fast(d[0]), rcp_fast(d[1])))), p + j);
+            get(mul(m2, im2), x);
+            get(mul(q2, is2), y);
+#pragma unroll
+            for (int w = 0; w < 2; w++) {
+                uint32_t rm, rs;
+                random_bits(hash + (uint32_t)(u * 128 + j + w) * 0x9E3779B1u, rm, rs);
+                // 16 x + r: the code's bits 20 to 26 come to 24 to 30, and the sign goes back to 31
+                a[j + w] = (__float_as_uint(x[w]) * 16u + rm) | (__float_as_uint(x[w]) & 0x80000000u);
+                b[j + w] = __float_as_uint(y[w]) * 16u + rs;
+                if (v[k + w] > 0.f) b[j + w] = max(b[j + w], 1u << 24);
+            }
         }
-        store4((P*)e.p + i, p + 4 * u);
+        store4((P*)e.p + i, p);
         *(uint32_t*)((uint8_t*)e.m + i) = top_bytes(a);
         *(uint32_t*)((uint8_t*)e.v + i) = top_bytes(b);
-        if (e.copy) store4((bf16*)e.copy + i, p + 4 * u);
+        if (e.copy) store4((bf16*)e.copy + i, p);
     }
     if ((threadIdx.x & 31) == 0) {
         e.m_exp[block] = (uint8_t)nm;
@@ -420,19 +514,38 @@ __device__ __forceinline__ bool adamw8_block(const Entry& e, int64_t block, cons
 }
 
 template <typename P, typename G, int CAP>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm) adamw8_kernel(const __grid_constant__ Table<CAP> t) {
-    const Step s = step_of(t.h);
+__global__ void __launch_bounds__(kThreads, kCtasPerSm8) adamw8_kernel(const __grid_constant__ Table<CAP> t) {
+    // the next block's loads are in flight while this one is computed
     const int64_t chunks = t.start[t.n];
-    int k = find(t, blockIdx.x);
-    for (int64_t c = blockIdx.x; c < chunks; c += gridDim.x) {
-        k = advance(t, k, c);
-        const Entry& e = t.e[k];
-        const bool vec = t.vec[k];
-        const int64_t block = (c - t.start[k]) * (kChunk / kBlock) + threadIdx.x / 32;
+    int64_t c = blockIdx.x;
+    int k = find(t, c);
+    auto block_of = [&](int64_t c, int k) { return (c - t.start[k]) * (kChunk / kBlock) + threadIdx.x / 32; };
+    auto whole = [&](int64_t block, int k) { return t.vec[k] && (block + 1) * kBlock <= t.e[k].n; };
+    int64_t block = block_of(c, k);
+    BlockIn<P, G> in, next;
+    bool full = whole(block, k);
+    if (full) in.load(t.e[k], block);
+    const Step s = step_of(t.h);
+    while (true) {
+        const int64_t c2 = c + gridDim.x;
+        int k2 = k;
+        int64_t block2 = 0;
+        bool full2 = false;
+        if (c2 < chunks) {
+            k2 = advance(t, k, c2);
+            block2 = block_of(c2, k2);
+            full2 = whole(block2, k2);
+            if (full2) next.load(t.e[k2], block2);
+        }
         const uint32_t key = mix(s.key ^ (t.h.first + k));
-        if (block * kBlock >= e.n) continue;   // the whole warp
-        if (vec && (block + 1) * kBlock <= e.n && adamw8_block<P, G>(e, block, t.h, s, key)) continue;
-        adamw8_odd_block<P, G>(e, block, vec, t.h, s, key);
+        if (!(full && adamw8_block<P, G>(in, t.e[k], block, t.h, s, key)) && block * kBlock < t.e[k].n)
+            adamw8_odd_block<P, G>(t.e[k], block, t.vec[k], t.h, s, key);
+        if (c2 >= chunks) break;
+        c = c2;
+        k = k2;
+        block = block2;
+        full = full2;
+        in = next;
     }
 }
 
@@ -523,8 +636,8 @@ int64_t fill(Table<CAP>& t, const Entry* e, const uint8_t* vec, int count, int c
     return t.start[count];
 }
 
-unsigned grid_for(tb_ctx* ctx, int64_t chunks) {
-    const int64_t cap = (int64_t)ctx->num_sms * kCtasPerSm;
+unsigned grid_for(tb_ctx* ctx, int64_t chunks, int ctas = kCtasPerSm) {
+    const int64_t cap = (int64_t)ctx->num_sms * ctas;
     return (unsigned)(chunks < cap ? chunks : cap);
 }
 
@@ -537,7 +650,7 @@ int adamw_launch(tb_ctx* ctx, int bits, const Entry* e, const uint8_t* vec, int 
     if (!chunks) return TB_OK;
     t.h = h;
     return launch(ctx, bits == 8 ? "adamw8" : "adamw", bits == 8 ? adamw8_kernel<P, G, CAP> : adamw_kernel<P, G, CAP>,
-                  dim3(grid_for(ctx, chunks)), dim3(kThreads), 0, t);
+                  dim3(grid_for(ctx, chunks, bits == 8 ? kCtasPerSm8 : kCtasPerSm)), dim3(kThreads), 0, t);
 }
 
 template <typename G, int CAP>
