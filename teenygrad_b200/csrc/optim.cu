@@ -39,11 +39,14 @@ namespace {
 
 using bf16 = __nv_bfloat16;
 
+constexpr int kBlock = 256;       // elements that share an exponent: one warp, 8 a lane
 constexpr int kThreads = 256;
 constexpr int kChunk = 2048;      // elements of one tensor that a CTA takes at a time
 constexpr int kNormChunk = 8192;  // the same of the gradient norm
-constexpr int kBlock = 256;       // elements that share an exponent: one warp, 8 a lane
-constexpr int kCtasPerSm = 4, kCtasPerSm8 = 2;
+constexpr int kCtasPerSm = 4;
+constexpr int kUnit8 = 2 * kBlock;                // 8-bit: what a warp takes at a time
+constexpr int kThreads8 = 128, kCtasPerSm8 = 5;
+constexpr int kChunk8 = kThreads8 / 32 * kUnit8;
 
 // Tensors a launch's parameters hold: 4 KB of them cost a launch nothing, 32 KB
 // some microseconds, so models of few tensors take the small table.
@@ -73,8 +76,9 @@ struct Hyper {
 template <int CAP>
 struct Table {
     Entry e[CAP];
-    int64_t start[CAP + 1];   // first chunk of each tensor; the last entry is the number of chunks
-    uint8_t vec[CAP];         // the tensor's addresses allow vector accesses
+    int start[CAP + 1];   // first chunk of each tensor; the last entry is the number of chunks
+    int whole[CAP];       // units of kUnit8 that are whole and at aligned addresses
+    uint8_t vec[CAP];     // the tensor's addresses allow vector accesses
     int n;
     Hyper h;
 };
@@ -83,7 +87,7 @@ static_assert(sizeof(Table<kLargeTable>) <= 32764 - 256, "fits the parameter spa
 
 // The tensor that holds a chunk.
 template <int CAP>
-__device__ __forceinline__ int find(const Table<CAP>& t, int64_t chunk) {
+__device__ __forceinline__ int find(const Table<CAP>& t, int chunk) {
     int lo = 0, hi = t.n;
     while (hi - lo > 1) {
         const int mid = (lo + hi) / 2;
@@ -96,7 +100,7 @@ __device__ __forceinline__ int find(const Table<CAP>& t, int64_t chunk) {
 // The same for a chunk at or after one that tensor k holds: the grid's stride passes
 // few tensors at a time.
 template <int CAP>
-__device__ __forceinline__ int advance(const Table<CAP>& t, int k, int64_t chunk) {
+__device__ __forceinline__ int advance(const Table<CAP>& t, int k, int chunk) {
     while (t.start[k + 1] <= chunk) k++;
     return k;
 }
@@ -203,13 +207,13 @@ template <typename P, typename G, int CAP>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) adamw_kernel(const __grid_constant__ Table<CAP> t) {
     const Step s = step_of(t.h);
     const float b1 = t.h.beta1, b2 = t.h.beta2, r1 = t.h.rest1, r2 = t.h.rest2;
-    const int64_t chunks = t.start[t.n];
+    const int chunks = t.start[t.n];
     int k = find(t, blockIdx.x);
-    for (int64_t c = blockIdx.x; c < chunks; c += gridDim.x) {
+    for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
         k = advance(t, k, c);
         const Entry& e = t.e[k];
         const bool vec = t.vec[k];
-        const int64_t n = e.n, i0 = (c - t.start[k]) * kChunk + threadIdx.x * 4;
+        const int64_t n = e.n, i0 = (int64_t)(c - t.start[k]) * kChunk + threadIdx.x * 4;
         P* pp = (P*)e.p;
         const G* pg = (const G*)e.g;
         float *pm = (float*)e.m, *pv = (float*)e.v;
@@ -300,10 +304,8 @@ __device__ __forceinline__ void decode4(uint32_t w, float* v) {
     v[0] = x.x; v[1] = x.y; v[2] = y.x; v[3] = y.y;
 }
 
-// The block's exponent for its largest value 2^e (1 + f).
-__device__ __forceinline__ int block_exponent(int e) { return max(e + 120, 0); }
-// floor(log2) of a float's bits, subnormal ones among them; for zero less than any exponent, and its half too.
-__device__ __forceinline__ int log2_of(uint32_t u) { return u >> 23 ? (int)(u >> 23) - 127 : u ? -118 - __clz(u) : -300; }
+// The block's exponent for its largest value's bits: that of its binade, less 7.
+__device__ __forceinline__ int block_exponent(uint32_t top) { return (int)max(top >> 23, 7u) - 7; }
 
 // Codes.  x is scaled to put the code's smallest normal value, 2^-6, on f32's, 2^-126: then
 // the code is the f32's bits 20 to 26, in the subnormal range too, and what lies below them
@@ -368,8 +370,8 @@ __device__ __noinline__ void adamw8_odd_block(const Entry& e, int64_t block, boo
             tv = max(tv, finite_bits(v[j]));
         }
     }
-    const int nm = block_exponent(log2_of(__reduce_max_sync(0xffffffffu, tm)));
-    const int ns = block_exponent(log2_of(__reduce_max_sync(0xffffffffu, tv)));
+    const int nm = block_exponent(__reduce_max_sync(0xffffffffu, tm));
+    const int ns = block_exponent(__reduce_max_sync(0xffffffffu, tv));
 #pragma unroll
     for (int u = 0; u < 2; u++) {
         const int64_t i = place(block, u);
@@ -392,65 +394,55 @@ __device__ __noinline__ void adamw8_odd_block(const Entry& e, int64_t block, boo
     }
 }
 
-// Four values as they lie in memory.
-template <typename T>
-struct Raw4;
-template <>
-struct Raw4<float> {
-    float4 a;
-    __device__ __forceinline__ void load(const float* p) { a = *reinterpret_cast<const float4*>(p); }
-    __device__ __forceinline__ void get(float* v) const { v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; }
-};
-template <>
-struct Raw4<bf16> {
-    uint2 a;
-    __device__ __forceinline__ void load(const bf16* p) { a = *reinterpret_cast<const uint2*>(p); }
-    __device__ __forceinline__ void get(float* v) const {
-        v[0] = bf16_lo(a.x); v[1] = bf16_hi(a.x); v[2] = bf16_lo(a.y); v[3] = bf16_hi(a.y);
-    }
+// What a step reads of a unit, on its way through shared memory.
+template <typename P, typename G>
+struct alignas(16) UnitIn {
+    P p[kUnit8];
+    G g[kUnit8];
+    uint8_t m[kUnit8], v[kUnit8];
 };
 
-// What a step reads of a block.
+__device__ __forceinline__ void copy16(void* smem, const void* global) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(smem)), "l"(global) : "memory");
+}
+
+// The whole warp copies a unit in, 16 bytes a lane at a time.
 template <typename P, typename G>
-struct BlockIn {
-    Raw4<P> p[2];
-    Raw4<G> g[2];
-    uint32_t cm[2], cs[2];
-    uint8_t em, es;
-    __device__ __forceinline__ void load(const Entry& e, int64_t block) {
+__device__ __forceinline__ void fetch(UnitIn<P, G>& in, const Entry& e, int unit) {
+    const int lane = threadIdx.x & 31;
+    auto part = [&](void* to, const void* from, int bytes) {
+        const char* at = (const char*)from + (int64_t)unit * bytes + lane * 16;
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const int64_t i = place(block, u);
-            p[u].load((const P*)e.p + i);
-            g[u].load((const G*)e.g + i);
-            cm[u] = *(const uint32_t*)((const uint8_t*)e.m + i);
-            cs[u] = *(const uint32_t*)((const uint8_t*)e.v + i);
-        }
-        em = e.m_exp[block];
-        es = e.v_exp[block];
-    }
-};
+        for (int o = 0; o < bytes; o += 512) copy16((char*)to + o + lane * 16, at + o);
+    };
+    part(in.p, e.p, sizeof(in.p));
+    part(in.g, e.g, sizeof(in.g));
+    part(in.m, e.m, sizeof(in.m));
+    part(in.v, e.v, sizeof(in.v));
+}
 
-// A whole block at aligned addresses; false, with nothing written, where it is not a common
-// one.  The common case folds the exponents into the betas (exact, as they are powers of two)
-// and takes the hardware's square root (2^-23), which flushes what is under 2^-126.
+// Block b of a whole unit at aligned addresses; false, with nothing written, where it is not a
+// common one.  The common case folds the exponents into the betas (exact, as they are powers of
+// two) and takes the hardware's square root (2^-23), which flushes what is under 2^-126.
 template <typename P, typename G>
-__device__ __forceinline__ bool adamw8_block(const BlockIn<P, G>& in, const Entry& e, int64_t block, const Hyper& h,
-                                             const Step& s, uint32_t key) {
-    const int64_t i0 = place(block, 0);
-    const int em = in.em, es = in.es;
+__device__ __forceinline__ bool adamw8_block(const UnitIn<P, G>& in, int b, uint32_t em, uint32_t es, const Entry& e,
+                                             int unit, const Hyper& h, const Step& s, uint32_t key) {
+    const int at = b * kBlock + (threadIdx.x & 31) * 4;
     // m beta1 = code * bm and s^2 beta2 = code^2 * bs
-    const float ds = power(es - 127), bm = power(em - 127) * h.beta1, bs = ds * ds * h.beta2;
+    const float ds = __uint_as_float(es << 23), bm = __uint_as_float(em << 23) * h.beta1, bs = ds * ds * h.beta2;
     const F2 bm2 = f2(bm, bm), bs2 = f2(bs, bs), scale2 = f2(s.scale, s.scale), r1 = f2(h.rest1, h.rest1),
              r2 = f2(h.rest2, h.rest2);
     float m[8], v[8];
     float top_m = 0.f, top_v = 0.f;
+    uint32_t codes = 0;
 #pragma unroll
     for (int u = 0; u < 2; u++) {
         float g[4];
-        decode4(in.cm[u], m + 4 * u);
-        decode4(in.cs[u], v + 4 * u);
-        in.g[u].get(g);
+        const uint32_t cm = *(const uint32_t*)(in.m + u * 128 + at), cs = *(const uint32_t*)(in.v + u * 128 + at);
+        decode4(cm, m + 4 * u);
+        decode4(cs, v + 4 * u);
+        codes |= cm | cs;
+        load4(in.g + u * 128 + at, g);
 #pragma unroll
         for (int j = 0; j < 4; j += 2) {
             const int k = 4 * u + j;
@@ -463,25 +455,26 @@ __device__ __forceinline__ bool adamw8_block(const BlockIn<P, G>& in, const Entr
     }
     const uint32_t tm = __reduce_max_sync(0xffffffffu, __float_as_uint(top_m));
     const uint32_t tv = __reduce_max_sync(0xffffffffu, __float_as_uint(top_v));
-    // Finite moments, under 2^37 (2^(127 - exponent + kCodeScale) has to be a number); held exponents whose
-    // products with a code are normal numbers, or codes that are all 0 (a new tensor's); a largest root above
-    // 2^-42, next to which a flushed one rounds as its own value does, or none; and an eps that a flushed root
-    // can do with.
-    const bool fresh = !(in.cm[0] | in.cm[1] | in.cs[0] | in.cs[1]);
-    if (!(tm < 164u << 23 && tv < 201u << 23 && ((em >= 32 && es >= 84) || __all_sync(0xffffffffu, fresh)) &&
+    // Moments under 2^14, so that the scale below is a normal number (what is not finite is above); held exponents
+    // whose products with a code are normal numbers, or codes that are all 0 (a new tensor's); a largest root above
+    // 2^-42, next to which a flushed one rounds as its own value does, or none; and an eps that a flushed root can
+    // do with.
+    if (!(tm < 141u << 23 && tv < 155u << 23 && ((em >= 32 && es >= 84) || __all_sync(0xffffffffu, !codes)) &&
           (tv >= 43u << 23 || tv == 0) && s.eps > 1e-30f))
         return false;
-    const int nm = block_exponent(log2_of(tm)), ns = block_exponent(log2_of(tv) >> 1);   // no root rounds up to a power of two
-    const float im = power(127 + kCodeScale - nm), is = power(127 + kCodeScale - ns);
+    // exponents of the largest value's binade, less 7; that of a root is half its square's (none rounds up to a power of two)
+    const uint32_t nm = max(tm >> 23, 7u) - 7u, ns = tv ? ((tv >> 23) + 113u) >> 1 : 0u;
+    const float im = __uint_as_float((134u - nm) << 23), is = __uint_as_float((134u - ns) << 23);   // 2^(127 + kCodeScale - n)
     const F2 im2 = f2(im, im), is2 = f2(is, is), root2 = f2(s.root, s.root), eps2 = f2(s.eps, s.eps),
              rate2 = f2(-s.rate, -s.rate), keep2 = f2(s.keep, s.keep);
+    const int64_t i0 = (int64_t)unit * kUnit8 + at;
     const uint32_t hash = hash_of(key, i0);
 #pragma unroll
     for (int u = 0; u < 2; u++) {
         const int64_t i = i0 + u * 128;
         float p[4];
         uint32_t a[4], b[4];
-        in.p[u].get(p);
+        load4(in.p + u * 128 + at, p);
 #pragma unroll
         for (int j = 0; j < 4; j += 2) {
             const int k = 4 * u + j;
@@ -507,45 +500,69 @@ __device__ __forceinline__ bool adamw8_block(const BlockIn<P, G>& in, const Entr
         if (e.copy) store4((bf16*)e.copy + i, p);
     }
     if ((threadIdx.x & 31) == 0) {
-        e.m_exp[block] = (uint8_t)nm;
-        e.v_exp[block] = (uint8_t)ns;
+        e.m_exp[(int64_t)unit * 2 + b] = (uint8_t)nm;
+        e.v_exp[(int64_t)unit * 2 + b] = (uint8_t)ns;
     }
     return true;
 }
 
+// Each warp has two units of its own in shared memory: asynchronous copies fill one while it
+// computes the other.
 template <typename P, typename G, int CAP>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm8) adamw8_kernel(const __grid_constant__ Table<CAP> t) {
-    // the next block's loads are in flight while this one is computed
-    const int64_t chunks = t.start[t.n];
-    int64_t c = blockIdx.x;
-    int k = find(t, c);
-    auto block_of = [&](int64_t c, int k) { return (c - t.start[k]) * (kChunk / kBlock) + threadIdx.x / 32; };
-    auto whole = [&](int64_t block, int k) { return t.vec[k] && (block + 1) * kBlock <= t.e[k].n; };
-    int64_t block = block_of(c, k);
-    BlockIn<P, G> in, next;
-    bool full = whole(block, k);
-    if (full) in.load(t.e[k], block);
+__global__ void __launch_bounds__(kThreads8, kCtasPerSm8) adamw8_kernel(const __grid_constant__ Table<CAP> t) {
+    __shared__ UnitIn<P, G> rings[kThreads8 / 32][2];
+    const int warp = threadIdx.x / 32, chunks = t.start[t.n];
+    UnitIn<P, G>* ring = rings[warp];
+    auto unit_of = [&](int c, int k) { return (c - t.start[k]) * (kChunk8 / kUnit8) + warp; };
+    auto exps_of = [&](int k, int unit) {   // m's in the low half, the first block's in its low byte
+        const uint8_t *m = t.e[k].m_exp + (int64_t)unit * 2, *v = t.e[k].v_exp + (int64_t)unit * 2;
+        return m[0] | m[1] << 8 | (uint32_t)v[0] << 16 | (uint32_t)v[1] << 24;
+    };
+    int c = blockIdx.x, k = find(t, c), unit = unit_of(c, k), stage = 0;
+    bool whole = unit < t.whole[k];
+    uint32_t exps = 0;
+    if (whole) {
+        fetch(ring[0], t.e[k], unit);
+        exps = exps_of(k, unit);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
     const Step s = step_of(t.h);
+    uint32_t key = mix(s.key ^ (t.h.first + k));
     while (true) {
-        const int64_t c2 = c + gridDim.x;
-        int k2 = k;
-        int64_t block2 = 0;
-        bool full2 = false;
+        const int c2 = c + gridDim.x;
+        int k2 = k, unit2 = 0;
+        bool whole2 = false;
+        uint32_t exps2 = 0;
         if (c2 < chunks) {
             k2 = advance(t, k, c2);
-            block2 = block_of(c2, k2);
-            full2 = whole(block2, k2);
-            if (full2) next.load(t.e[k2], block2);
+            unit2 = unit_of(c2, k2);
+            whole2 = unit2 < t.whole[k2];
+            if (whole2) {
+                fetch(ring[stage ^ 1], t.e[k2], unit2);
+                exps2 = exps_of(k2, unit2);
+            }
         }
-        const uint32_t key = mix(s.key ^ (t.h.first + k));
-        if (!(full && adamw8_block<P, G>(in, t.e[k], block, t.h, s, key)) && block * kBlock < t.e[k].n)
-            adamw8_odd_block<P, G>(t.e[k], block, t.vec[k], t.h, s, key);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        __syncwarp();
+        const Entry& e = t.e[k];
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            const int64_t block = (int64_t)unit * 2 + b;
+            if (whole && adamw8_block<P, G>(ring[stage], b, exps >> 8 * b & 0xff, exps >> (16 + 8 * b) & 0xff, e, unit, t.h,
+                                            s, key))
+                continue;
+            if (block * kBlock < e.n) adamw8_odd_block<P, G>(e, block, t.vec[k], t.h, s, key);
+        }
         if (c2 >= chunks) break;
+        __syncwarp();   // all have read the stage that the next copy fills
+        if (k2 != k) key = mix(s.key ^ (t.h.first + k2));
         c = c2;
         k = k2;
-        block = block2;
-        full = full2;
-        in = next;
+        unit = unit2;
+        whole = whole2;
+        exps = exps2;
+        stage ^= 1;
     }
 }
 
@@ -568,13 +585,13 @@ template <typename G, int CAP>
 __global__ void __launch_bounds__(kThreads) sumsq_kernel(const __grid_constant__ Table<CAP> t, double* __restrict__ part) {
     constexpr int V = 16 / sizeof(G), L = kNormChunk / kThreads / V;
     __shared__ double red[kThreads / 32];
-    const int64_t chunks = t.start[t.n];
+    const int chunks = t.start[t.n];
     double acc = 0.0;
     int k = find(t, blockIdx.x);
-    for (int64_t c = blockIdx.x; c < chunks; c += gridDim.x) {
+    for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
         k = advance(t, k, c);
         const G* g = (const G*)t.e[k].g;
-        const int64_t i0 = (c - t.start[k]) * kNormChunk, n = t.e[k].n;
+        const int64_t i0 = (int64_t)(c - t.start[k]) * kNormChunk, n = t.e[k].n;
         float s = 0.f;
         if (t.vec[k] && i0 + kNormChunk <= n) {
             uint4 a[L];
@@ -623,15 +640,19 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const double* __restrict
 // ------------------------------------------------------------------- host --
 int64_t chunks_of(int64_t n, int chunk) { return (n + chunk - 1) / chunk; }
 
+// Elements in a list at most, so that chunks and units are counted in 32 bits.
+constexpr int64_t kMostElements = 1ll << 39;
+
 // Fills a table with the first tensors of a list; returns its chunks.
 template <int CAP>
-int64_t fill(Table<CAP>& t, const Entry* e, const uint8_t* vec, int count, int chunk) {
+int fill(Table<CAP>& t, const Entry* e, const uint8_t* vec, int count, int chunk) {
     t.n = count;
     t.start[0] = 0;
     for (int k = 0; k < count; k++) {
         t.e[k] = e[k];
         t.vec[k] = vec[k];
-        t.start[k + 1] = t.start[k] + chunks_of(e[k].n, chunk);
+        t.whole[k] = vec[k] ? (int)(e[k].n / kUnit8) : 0;
+        t.start[k + 1] = t.start[k] + (int)chunks_of(e[k].n, chunk);
     }
     return t.start[count];
 }
@@ -646,17 +667,19 @@ bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) &
 template <typename P, typename G, int CAP>
 int adamw_launch(tb_ctx* ctx, int bits, const Entry* e, const uint8_t* vec, int count, const Hyper& h) {
     Table<CAP> t;
-    const int64_t chunks = fill(t, e, vec, count, kChunk);
+    const int chunks = fill(t, e, vec, count, bits == 8 ? kChunk8 : kChunk);
     if (!chunks) return TB_OK;
     t.h = h;
-    return launch(ctx, bits == 8 ? "adamw8" : "adamw", bits == 8 ? adamw8_kernel<P, G, CAP> : adamw_kernel<P, G, CAP>,
-                  dim3(grid_for(ctx, chunks, bits == 8 ? kCtasPerSm8 : kCtasPerSm)), dim3(kThreads), 0, t);
+    if (bits == 8)
+        return launch(ctx, "adamw8", adamw8_kernel<P, G, CAP>, dim3(grid_for(ctx, chunks, kCtasPerSm8)), dim3(kThreads8), 0,
+                      t);
+    return launch(ctx, "adamw", adamw_kernel<P, G, CAP>, dim3(grid_for(ctx, chunks)), dim3(kThreads), 0, t);
 }
 
 template <typename G, int CAP>
 int sumsq_launch(tb_ctx* ctx, const Entry* e, const uint8_t* vec, int count, double* part) {
     Table<CAP> t;
-    const int64_t chunks = fill(t, e, vec, count, kNormChunk);
+    const int chunks = fill(t, e, vec, count, kNormChunk);
     t.h = Hyper{};
     // every launch writes its own row of partial sums, of one CTA where there is nothing to add
     return launch(ctx, "grad_norm", sumsq_kernel<G, CAP>, dim3(chunks ? grid_for(ctx, chunks) : 1u), dim3(kThreads), 0, t,
@@ -713,9 +736,12 @@ int tb_adamw_create(tb_ctx* ctx, int p_dtype, int g_dtype, int state_bits, const
     TB_REQUIRE(ctx, types, TB_ERR_UNSUPPORTED, "adamw: parameters and gradients f32 / f32, f32 / bf16 or bf16 / bf16");
     TB_REQUIRE(ctx, state_bits == 32 || state_bits == 8, TB_ERR_UNSUPPORTED, "adamw: moments in 32 or 8 bits");
     const size_t ps = p_dtype == TB_F32 ? 4 : 2, gs = g_dtype == TB_F32 ? 4 : 2, ms = state_bits / 8;
+    int64_t total = 0;
     for (int k = 0; k < n; k++) {
         const tb_adamw_tensor& t = tensors[k];
-        TB_REQUIRE(ctx, t.n >= 0 && t.n < (1ll << 48), TB_ERR_SHAPE, "adamw: tensor %d has %lld elements", k, (long long)t.n);
+        TB_REQUIRE(ctx, t.n >= 0 && t.n <= kMostElements - total, TB_ERR_SHAPE, "adamw: tensor %d has %lld elements", k,
+                   (long long)t.n);
+        total += t.n;
         if (!t.n) continue;
         TB_REQUIRE(ctx, t.p && t.g && t.m && t.v && (state_bits == 32 || (t.m_exp && t.v_exp)), TB_ERR_ARG,
                    "adamw: null pointer in tensor %d", k);
@@ -747,8 +773,10 @@ int tb_adamw_create(tb_ctx* ctx, int p_dtype, int g_dtype, int state_bits, const
     for (int k = 0; k < n; k++) {
         const tb_adamw_tensor& t = tensors[k];
         a->e[k] = {t.p, t.g, t.m, t.v, t.m_exp, t.v_exp, t.copy, t.n};
-        a->vec[k] = aligned(t.p, 4 * ps) && aligned(t.g, 4 * gs) && aligned(t.m, 4 * ms) && aligned(t.v, 4 * ms) &&
-                    aligned(t.copy, 8);
+        // four elements at a time; 16 bytes where blocks go through shared memory
+        a->vec[k] = state_bits == 8 ? aligned16(t.p) && aligned16(t.g) && aligned16(t.m) && aligned16(t.v) && aligned(t.copy, 8)
+                                    : aligned(t.p, 4 * ps) && aligned(t.g, 4 * gs) && aligned16(t.m) && aligned16(t.v) &&
+                                          aligned(t.copy, 8);
         const size_t cnt = (size_t)t.n, blocks = (cnt + kBlock - 1) / kBlock;
         add(t.p, cnt * ps, true);
         add(t.g, cnt * gs, false);
@@ -832,9 +860,11 @@ int tb_grad_norm(tb_ctx* ctx, int dtype, const void* const* grads, const int64_t
     if (dtype != TB_F32 && dtype != TB_BF16) return set_error(ctx, TB_ERR_UNSUPPORTED, "grad_norm: dtype %d", dtype);
     TB_REQUIRE(ctx, !scale || max_norm >= 0, TB_ERR_ARG, "grad_norm: max_norm >= 0");
     const size_t es = dtype == TB_F32 ? 4 : 2;
+    int64_t total = 0;
     for (int k = 0; k < n; k++) {
-        TB_REQUIRE(ctx, sizes[k] >= 0 && sizes[k] < (1ll << 48), TB_ERR_SHAPE, "grad_norm: tensor %d has %lld elements", k,
-                   (long long)sizes[k]);
+        TB_REQUIRE(ctx, sizes[k] >= 0 && sizes[k] <= kMostElements - total, TB_ERR_SHAPE, "grad_norm: tensor %d has %lld elements",
+                   k, (long long)sizes[k]);
+        total += sizes[k];
         TB_REQUIRE(ctx, grads[k] || !sizes[k], TB_ERR_ARG, "grad_norm: null pointer");
         TB_REQUIRE(ctx, aligned(grads[k], es), TB_ERR_ALIGN, "grad_norm: tensor %d is not aligned to its type", k);
     }
