@@ -45,7 +45,7 @@ constexpr int kChunk = 2048;      // elements of one tensor that a CTA takes at 
 constexpr int kNormChunk = 8192;  // the same of the gradient norm
 constexpr int kCtasPerSm = 4;
 constexpr int kUnit8 = 2 * kBlock;                // 8-bit: what a warp takes at a time
-constexpr int kThreads8 = 128, kCtasPerSm8 = 5;
+constexpr int kThreads8 = 64;
 constexpr int kChunk8 = kThreads8 / 32 * kUnit8;
 
 // Tensors a launch's parameters hold: 4 KB of them cost a launch nothing, 32 KB
@@ -201,6 +201,14 @@ __device__ __forceinline__ float stepped(float p, float m, float root_v, const S
     float q;
     asm("div.approx.ftz.f32 %0, %1, %2;" : "=f"(q) : "f"(s.rate * m), "f"(root_v * s.root + s.eps));
     return p * s.keep - q;
+}
+
+// CTAs an SM: as many as keep HBM busy, since more of them cost DRAM rows.  1e9 parameters, with 2 / 3 / 4 CTAs:
+// f32 and f32 gradients 4.35 / 4.52 / 4.54 ms, bf16 gradients 4.72 / 4.12 / 4.28 and with the copy 5.01 / 4.55 / 4.62,
+// bf16 and bf16 4.38 / 3.70 / 3.50.  (The floors are 4.34, 4.03, 4.34 and 3.41.)
+template <typename P, typename G>
+constexpr int adamw_ctas() {
+    return sizeof(P) == 2 ? 4 : sizeof(G) == 2 ? 3 : 2;
 }
 
 template <typename P, typename G, int CAP>
@@ -506,11 +514,26 @@ __device__ __forceinline__ bool adamw8_block(const UnitIn<P, G>& in, int b, uint
     return true;
 }
 
-// Each warp has two units of its own in shared memory: asynchronous copies fill one while it
-// computes the other.
+// How many units a warp's ring holds and how many CTAs an SM.  With f32 parameters HBM is the
+// bound: 12 warps of 3 or 4 units (5 KB or 4 KB) keep enough in flight, and more of them cost
+// DRAM rows (1e9 parameters, bf16 gradients and a copy: 6 CTAs of 4 units 2.49 ms, 8 of 3 2.93,
+// 10 of 2 2.93, 4 of 4 3.09).  With bf16 parameters instruction issue is: as many warps as the
+// registers allow (10 CTAs of 2 units 1.99 ms, 6 of 4 2.31).  An odd number of CTAs leaves
+// sub-partitions of the SM uneven.
+template <typename P, typename G>
+struct Ring8 {
+    static constexpr bool wide = sizeof(P) == 4;
+    static constexpr int stages = !wide ? 2 : sizeof(G) == 4 ? 3 : 4;
+    static constexpr int ctas = wide ? 6 : 10;
+    static_assert(ctas * (sizeof(UnitIn<P, G>) * stages * (kThreads8 / 32) + 1024) <= 227 * 1024, "fits the SM");
+};
+
+// Each warp has a ring of units of its own in shared memory: asynchronous copies fill
+// the others while it computes one.
 template <typename P, typename G, int CAP>
-__global__ void __launch_bounds__(kThreads8, kCtasPerSm8) adamw8_kernel(const __grid_constant__ Table<CAP> t) {
-    __shared__ UnitIn<P, G> rings[kThreads8 / 32][2];
+__global__ void __launch_bounds__(kThreads8, 10) adamw8_kernel(const __grid_constant__ Table<CAP> t) {
+    constexpr int S = Ring8<P, G>::stages;
+    __shared__ UnitIn<P, G> rings[kThreads8 / 32][S];
     const int warp = threadIdx.x / 32, chunks = t.start[t.n];
     UnitIn<P, G>* ring = rings[warp];
     auto unit_of = [&](int c, int k) { return (c - t.start[k]) * (kChunk8 / kUnit8) + warp; };
@@ -518,51 +541,57 @@ __global__ void __launch_bounds__(kThreads8, kCtasPerSm8) adamw8_kernel(const __
         const uint8_t *m = t.e[k].m_exp + (int64_t)unit * 2, *v = t.e[k].v_exp + (int64_t)unit * 2;
         return m[0] | m[1] << 8 | (uint32_t)v[0] << 16 | (uint32_t)v[1] << 24;
     };
-    int c = blockIdx.x, k = find(t, c), unit = unit_of(c, k), stage = 0;
-    bool whole = unit < t.whole[k];
-    uint32_t exps = 0;
-    if (whole) {
-        fetch(ring[0], t.e[k], unit);
-        exps = exps_of(k, unit);
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    const Step s = step_of(t.h);
-    uint32_t key = mix(s.key ^ (t.h.first + k));
-    while (true) {
-        const int c2 = c + gridDim.x;
-        int k2 = k, unit2 = 0;
-        bool whole2 = false;
-        uint32_t exps2 = 0;
-        if (c2 < chunks) {
-            k2 = advance(t, k, c2);
-            unit2 = unit_of(c2, k2);
-            whole2 = unit2 < t.whole[k2];
-            if (whole2) {
-                fetch(ring[stage ^ 1], t.e[k2], unit2);
-                exps2 = exps_of(k2, unit2);
+    // the units in flight, the present one first
+    int ks[S] = {}, units[S] = {};
+    uint32_t exps[S] = {};
+    bool whole[S] = {};
+    int c = blockIdx.x, ahead = c;
+    auto start = [&](int i, int stage) {   // the next unit's copies, its place in slot i
+        whole[i] = false;
+        if (ahead < chunks) {
+            ks[i] = i ? advance(t, ks[i - 1], ahead) : find(t, ahead);
+            units[i] = unit_of(ahead, ks[i]);
+            whole[i] = units[i] < t.whole[ks[i]];
+            if (whole[i]) {
+                fetch(ring[stage], t.e[ks[i]], units[i]);
+                exps[i] = exps_of(ks[i], units[i]);
             }
+            ahead += gridDim.x;
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
-        asm volatile("cp.async.wait_group 1;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < S - 1; i++) start(i, i);
+    const Step s = step_of(t.h);
+    int known = -1, stage = 0;
+    uint32_t key = 0;
+    for (; c < chunks; c += gridDim.x) {
+        start(S - 1, stage ? stage - 1 : S - 1);
+        asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory");
         __syncwarp();
+        const int k = ks[0];
         const Entry& e = t.e[k];
+        if (k != known) {
+            known = k;
+            key = mix(s.key ^ (t.h.first + k));
+        }
 #pragma unroll
         for (int b = 0; b < 2; b++) {
-            const int64_t block = (int64_t)unit * 2 + b;
-            if (whole && adamw8_block<P, G>(ring[stage], b, exps >> 8 * b & 0xff, exps >> (16 + 8 * b) & 0xff, e, unit, t.h,
-                                            s, key))
+            const int64_t block = (int64_t)units[0] * 2 + b;
+            if (whole[0] && adamw8_block<P, G>(ring[stage], b, exps[0] >> 8 * b & 0xff, exps[0] >> (16 + 8 * b) & 0xff, e,
+                                               units[0], t.h, s, key))
                 continue;
             if (block * kBlock < e.n) adamw8_odd_block<P, G>(e, block, t.vec[k], t.h, s, key);
         }
-        if (c2 >= chunks) break;
         __syncwarp();   // all have read the stage that the next copy fills
-        if (k2 != k) key = mix(s.key ^ (t.h.first + k2));
-        c = c2;
-        k = k2;
-        unit = unit2;
-        whole = whole2;
-        exps = exps2;
-        stage ^= 1;
+        stage = stage + 1 < S ? stage + 1 : 0;
+#pragma unroll
+        for (int i = 0; i + 1 < S; i++) {
+            ks[i] = ks[i + 1];
+            units[i] = units[i + 1];
+            exps[i] = exps[i + 1];
+            whole[i] = whole[i + 1];
+        }
     }
 }
 
@@ -671,9 +700,9 @@ int adamw_launch(tb_ctx* ctx, int bits, const Entry* e, const uint8_t* vec, int 
     if (!chunks) return TB_OK;
     t.h = h;
     if (bits == 8)
-        return launch(ctx, "adamw8", adamw8_kernel<P, G, CAP>, dim3(grid_for(ctx, chunks, kCtasPerSm8)), dim3(kThreads8), 0,
+        return launch(ctx, "adamw8", adamw8_kernel<P, G, CAP>, dim3(grid_for(ctx, chunks, Ring8<P, G>::ctas)), dim3(kThreads8), 0,
                       t);
-    return launch(ctx, "adamw", adamw_kernel<P, G, CAP>, dim3(grid_for(ctx, chunks)), dim3(kThreads), 0, t);
+    return launch(ctx, "adamw", adamw_kernel<P, G, CAP>, dim3(grid_for(ctx, chunks, adamw_ctas<P, G>())), dim3(kThreads), 0, t);
 }
 
 template <typename G, int CAP>

@@ -662,7 +662,7 @@ class AdamW:
 
     def __init__(self, params, grads, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32,
                  copies=None, seed=0, state=None, step_count=0, capturable=False):
-        self._handle = None
+        self._handle, self._destroy = None, lib().tb_adamw_destroy   # of use when the interpreter ends, too
         self.params, self.grads = list(params), list(grads)
         self.copies = None if copies is None else list(copies)
         self.lr, self.state_bits = lr, state_bits
@@ -718,7 +718,7 @@ class AdamW:
 
     def __del__(self):
         if getattr(self, "_handle", None):
-            lib().tb_adamw_destroy(self._handle)
+            self._destroy(self._handle)
             self._handle = None
 
     @property
