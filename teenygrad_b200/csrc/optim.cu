@@ -429,87 +429,99 @@ __device__ __forceinline__ void fetch(UnitIn<P, G>& in, const Entry& e, int unit
     part(in.v, e.v, sizeof(in.v));
 }
 
-// Block b of a whole unit at aligned addresses; false, with nothing written, where it is not a
-// common one.  The common case folds the exponents into the betas (exact, as they are powers of
-// two) and takes the hardware's square root (2^-23), which flushes what is under 2^-126.
+// The two blocks of a whole unit at aligned addresses; false, with nothing written, where one is
+// not a common one.  The common case folds the exponents into the betas (exact, as they are powers
+// of two) and takes the hardware's square root (2^-23), which flushes what is under 2^-126.
+// exps: m's exponents in bytes 0 and 1, s's in 2 and 3.
 template <typename P, typename G>
-__device__ __forceinline__ bool adamw8_block(const UnitIn<P, G>& in, int b, uint32_t em, uint32_t es, const Entry& e,
-                                             int unit, const Hyper& h, const Step& s, uint32_t key) {
-    const int at = b * kBlock + (threadIdx.x & 31) * 4;
-    // m beta1 = code * bm and s^2 beta2 = code^2 * bs
-    const float ds = __uint_as_float(es << 23), bm = __uint_as_float(em << 23) * h.beta1, bs = ds * ds * h.beta2;
-    const F2 bm2 = f2(bm, bm), bs2 = f2(bs, bs), scale2 = f2(s.scale, s.scale), r1 = f2(h.rest1, h.rest1),
-             r2 = f2(h.rest2, h.rest2);
-    float m[8], v[8];
-    float top_m = 0.f, top_v = 0.f;
-    uint32_t codes = 0;
+__device__ __forceinline__ bool adamw8_unit(const UnitIn<P, G>& in, uint32_t exps, const Entry& e, int unit, const Hyper& h,
+                                            const Step& s, uint32_t key) {
+    constexpr int B = 2;
+    const int at = (threadIdx.x & 31) * 4;
+    const F2 scale2 = f2(s.scale, s.scale), r1 = f2(h.rest1, h.rest1), r2 = f2(h.rest2, h.rest2);
+    float m[8 * B], v[8 * B];
+    uint32_t tm[B], tv[B];
+    bool common = s.eps > 1e-30f;   // a flushed root can do with that
 #pragma unroll
-    for (int u = 0; u < 2; u++) {
-        float g[4];
-        const uint32_t cm = *(const uint32_t*)(in.m + u * 128 + at), cs = *(const uint32_t*)(in.v + u * 128 + at);
-        decode4(cm, m + 4 * u);
-        decode4(cs, v + 4 * u);
-        codes |= cm | cs;
-        load4(in.g + u * 128 + at, g);
+    for (int b = 0; b < B; b++) {
+        // m beta1 = code * bm and s^2 beta2 = code^2 * bs
+        const uint32_t em = exps >> 8 * b & 0xff, es = exps >> 8 * (b + 2) & 0xff;
+        const float ds = __uint_as_float(es << 23), bm = __uint_as_float(em << 23) * h.beta1, bs = ds * ds * h.beta2;
+        const F2 bm2 = f2(bm, bm), bs2 = f2(bs, bs);
+        float top_m = 0.f, top_v = 0.f;
+        uint32_t codes = 0;
 #pragma unroll
-        for (int j = 0; j < 4; j += 2) {
-            const int k = 4 * u + j;
-            const F2 g2 = mul(f2(g[j], g[j + 1]), scale2), c2 = f2(v[k], v[k + 1]);
-            sums(mul(f2(m[k], m[k + 1]), bm2), mul(g2, r1), m + k);
-            sums(mul(mul(c2, c2), bs2), mul(mul(g2, g2), r2), v + k);
-            top_m = largest(top_m, m[k], m[k + 1]);
-            top_v = largest(top_v, v[k], v[k + 1]);
+        for (int u = 0; u < 2; u++) {
+            const int o = b * kBlock + u * 128 + at;
+            float g[4];
+            const uint32_t cm = *(const uint32_t*)(in.m + o), cs = *(const uint32_t*)(in.v + o);
+            decode4(cm, m + 8 * b + 4 * u);
+            decode4(cs, v + 8 * b + 4 * u);
+            codes |= cm | cs;
+            load4(in.g + o, g);
+#pragma unroll
+            for (int j = 0; j < 4; j += 2) {
+                const int k = 8 * b + 4 * u + j;
+                const F2 g2 = mul(f2(g[j], g[j + 1]), scale2), c2 = f2(v[k], v[k + 1]);
+                sums(mul(f2(m[k], m[k + 1]), bm2), mul(g2, r1), m + k);
+                sums(mul(mul(c2, c2), bs2), mul(mul(g2, g2), r2), v + k);
+                top_m = largest(top_m, m[k], m[k + 1]);
+                top_v = largest(top_v, v[k], v[k + 1]);
+            }
         }
+        tm[b] = __reduce_max_sync(0xffffffffu, __float_as_uint(top_m));
+        tv[b] = __reduce_max_sync(0xffffffffu, __float_as_uint(top_v));
+        // Moments under 2^14, so that the scale below is a normal number (what is not finite is above); a largest
+        // root above 2^-42, next to which a flushed one rounds as its own value does, or none; and held exponents
+        // whose products with a code are normal numbers, or codes that are all 0 (a new tensor's).
+        common = common && tm[b] < 141u << 23 && tv[b] < 155u << 23 && (tv[b] >= 43u << 23 || tv[b] == 0) &&
+                 ((em >= 32 && es >= 84) || __all_sync(0xffffffffu, !codes));
     }
-    const uint32_t tm = __reduce_max_sync(0xffffffffu, __float_as_uint(top_m));
-    const uint32_t tv = __reduce_max_sync(0xffffffffu, __float_as_uint(top_v));
-    // Moments under 2^14, so that the scale below is a normal number (what is not finite is above); held exponents
-    // whose products with a code are normal numbers, or codes that are all 0 (a new tensor's); a largest root above
-    // 2^-42, next to which a flushed one rounds as its own value does, or none; and an eps that a flushed root can
-    // do with.
-    if (!(tm < 141u << 23 && tv < 155u << 23 && ((em >= 32 && es >= 84) || __all_sync(0xffffffffu, !codes)) &&
-          (tv >= 43u << 23 || tv == 0) && s.eps > 1e-30f))
-        return false;
-    // exponents of the largest value's binade, less 7; that of a root is half its square's (none rounds up to a power of two)
-    const uint32_t nm = max(tm >> 23, 7u) - 7u, ns = tv ? ((tv >> 23) + 113u) >> 1 : 0u;
-    const float im = __uint_as_float((134u - nm) << 23), is = __uint_as_float((134u - ns) << 23);   // 2^(127 + kCodeScale - n)
-    const F2 im2 = f2(im, im), is2 = f2(is, is), root2 = f2(s.root, s.root), eps2 = f2(s.eps, s.eps),
-             rate2 = f2(-s.rate, -s.rate), keep2 = f2(s.keep, s.keep);
+    if (!common) return false;
+    const F2 root2 = f2(s.root, s.root), eps2 = f2(s.eps, s.eps), rate2 = f2(-s.rate, -s.rate), keep2 = f2(s.keep, s.keep);
     const int64_t i0 = (int64_t)unit * kUnit8 + at;
     const uint32_t hash = hash_of(key, i0);
 #pragma unroll
-    for (int u = 0; u < 2; u++) {
-        const int64_t i = i0 + u * 128;
-        float p[4];
-        uint32_t a[4], b[4];
-        load4(in.p + u * 128 + at, p);
+    for (int b = 0; b < B; b++) {
+        // exponents of the largest value's binade, less 7; that of a root is half its square's (none rounds up to a
+        // power of two)
+        const uint32_t nm = max(tm[b] >> 23, 7u) - 7u, ns = tv[b] ? ((tv[b] >> 23) + 113u) >> 1 : 0u;
+        const float im = __uint_as_float((134u - nm) << 23), is = __uint_as_float((134u - ns) << 23);   // 2^(127 + kCodeScale - n)
+        const F2 im2 = f2(im, im), is2 = f2(is, is);
 #pragma unroll
-        for (int j = 0; j < 4; j += 2) {
-            const int k = 4 * u + j;
-            const F2 m2 = f2(m[k], m[k + 1]), q2 = f2(sqrt_fast(v[k]), sqrt_fast(v[k + 1]));
-            float d[2], x[2], y[2];
-            get(fma(q2, root2, eps2), d);
-            get(fma(f2(p[j], p[j + 1]), keep2, mul(mul(m2, rate2), f2(rcp_fast(d[0]), rcp_fast(d[1])))), p + j);
-            get(mul(m2, im2), x);
-            get(mul(q2, is2), y);
+        for (int u = 0; u < 2; u++) {
+            const int o = b * kBlock + u * 128;
+            float p[4];
+            uint32_t wm[4], ws[4];
+            load4(in.p + o + at, p);
 #pragma unroll
-            for (int w = 0; w < 2; w++) {
-                uint32_t rm, rs;
-                random_bits(hash + (uint32_t)(u * 128 + j + w) * 0x9E3779B1u, rm, rs);
-                // 16 x + r: the code's bits 20 to 26 come to 24 to 30, and the sign goes back to 31
-                a[j + w] = (__float_as_uint(x[w]) * 16u + rm) | (__float_as_uint(x[w]) & 0x80000000u);
-                b[j + w] = __float_as_uint(y[w]) * 16u + rs;
-                if (v[k + w] > 0.f) b[j + w] = max(b[j + w], 1u << 24);
+            for (int j = 0; j < 4; j += 2) {
+                const int k = 8 * b + 4 * u + j;
+                const F2 m2 = f2(m[k], m[k + 1]), q2 = f2(sqrt_fast(v[k]), sqrt_fast(v[k + 1]));
+                float d[2], x[2], y[2];
+                get(fma(q2, root2, eps2), d);
+                get(fma(f2(p[j], p[j + 1]), keep2, mul(mul(m2, rate2), f2(rcp_fast(d[0]), rcp_fast(d[1])))), p + j);
+                get(mul(m2, im2), x);
+                get(mul(q2, is2), y);
+#pragma unroll
+                for (int w = 0; w < 2; w++) {
+                    uint32_t rm, rs;
+                    random_bits(hash + (uint32_t)(o + j + w) * 0x9E3779B1u, rm, rs);
+                    // 16 x + r: the code's bits 20 to 26 come to 24 to 30, and the sign goes back to 31
+                    wm[j + w] = (__float_as_uint(x[w]) * 16u + rm) | (__float_as_uint(x[w]) & 0x80000000u);
+                    ws[j + w] = __float_as_uint(y[w]) * 16u + rs;
+                    if (v[k + w] > 0.f) ws[j + w] = max(ws[j + w], 1u << 24);
+                }
             }
+            store4((P*)e.p + i0 + o, p);
+            *(uint32_t*)((uint8_t*)e.m + i0 + o) = top_bytes(wm);
+            *(uint32_t*)((uint8_t*)e.v + i0 + o) = top_bytes(ws);
+            if (e.copy) store4((bf16*)e.copy + i0 + o, p);
         }
-        store4((P*)e.p + i, p);
-        *(uint32_t*)((uint8_t*)e.m + i) = top_bytes(a);
-        *(uint32_t*)((uint8_t*)e.v + i) = top_bytes(b);
-        if (e.copy) store4((bf16*)e.copy + i, p);
-    }
-    if ((threadIdx.x & 31) == 0) {
-        e.m_exp[(int64_t)unit * 2 + b] = (uint8_t)nm;
-        e.v_exp[(int64_t)unit * 2 + b] = (uint8_t)ns;
+        if ((threadIdx.x & 31) == 0) {
+            e.m_exp[(int64_t)unit * 2 + b] = (uint8_t)nm;
+            e.v_exp[(int64_t)unit * 2 + b] = (uint8_t)ns;
+        }
     }
     return true;
 }
@@ -531,7 +543,7 @@ struct Ring8 {
 // Each warp has a ring of units of its own in shared memory: asynchronous copies fill
 // the others while it computes one.
 template <typename P, typename G, int CAP>
-__global__ void __launch_bounds__(kThreads8, 10) adamw8_kernel(const __grid_constant__ Table<CAP> t) {
+__global__ void __launch_bounds__(kThreads8, Ring8<P, G>::ctas) adamw8_kernel(const __grid_constant__ Table<CAP> t) {
     constexpr int S = Ring8<P, G>::stages;
     __shared__ UnitIn<P, G> rings[kThreads8 / 32][S];
     const int warp = threadIdx.x / 32, chunks = t.start[t.n];
@@ -575,13 +587,10 @@ __global__ void __launch_bounds__(kThreads8, 10) adamw8_kernel(const __grid_cons
             known = k;
             key = mix(s.key ^ (t.h.first + k));
         }
-#pragma unroll
-        for (int b = 0; b < 2; b++) {
-            const int64_t block = (int64_t)units[0] * 2 + b;
-            if (whole[0] && adamw8_block<P, G>(ring[stage], b, exps[0] >> 8 * b & 0xff, exps[0] >> (16 + 8 * b) & 0xff, e,
-                                               units[0], t.h, s, key))
-                continue;
-            if (block * kBlock < e.n) adamw8_odd_block<P, G>(e, block, t.vec[k], t.h, s, key);
+        if (!(whole[0] && adamw8_unit(ring[stage], exps[0], e, units[0], t.h, s, key))) {
+#pragma unroll 1
+            for (int64_t block = (int64_t)units[0] * 2; block < (int64_t)units[0] * 2 + 2 && block * kBlock < e.n; block++)
+                adamw8_odd_block<P, G>(e, block, t.vec[k], t.h, s, key);
         }
         __syncwarp();   // all have read the stage that the next copy fills
         stage = stage + 1 < S ? stage + 1 : 0;
