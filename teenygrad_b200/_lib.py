@@ -31,6 +31,8 @@ class TeenyError(RuntimeError):
 _P, _I, _L, _D, _Z = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_double, ctypes.c_size_t
 # Entry points called with plain Python numbers.
 _ARGTYPES = {
+    "tb_set_stream": [_P, _P],
+    "tb_workspace_bytes": [_I, _I, _P, _I, _P],
     "tb_layernorm_fwd_train": [_P, _I, _P, _P, _P, _P, _P, _P, _L, _L, ctypes.c_float],
     "tb_layernorm_bwd": [_P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _I, _L, _L, _P, _Z],
     "tb_grad_norm": [_P, _I, _P, _P, _I, _P, _P, _D, _P, _Z],

@@ -7,16 +7,28 @@
 //   dx = rstd (a - c1 - xhat c2),  dw = sum_m dy xhat,  db = sum_m dy
 //
 // Bound by HBM: the forward moves x and y, the backward x, dy and dx, once
-// each.  A row lives in the registers of a group of TPR threads (a warp, or the
-// CTA), EPT elements a thread, so the mean, the centred variance and the output
-// come from one read; the groups walk the rows with the grid's stride and keep w
-// (and b) in registers.  In the backward each thread also keeps the f32 sums of
-// dw and db for its columns over all the rows it walks; the CTAs write them as
-// partial rows, and a second launch adds those in CTA order: no atomics, the
-// same bits on each run.  Rows longer than the registers hold take the kernels
-// that read a row more than once.
+// each.  A row belongs to a group of threads (a warp, or a CTA of as many as the
+// row needs), one or two 16-byte vectors a thread; the groups walk the rows with
+// the grid's stride and keep w (and b) in registers.  Each thread copies its own
+// vectors of the next rows into its own slots of a ring in shared memory
+// (cp.async: no registers, no barrier), so that rows are in flight while one is
+// reduced.  In the backward each thread also keeps the f32 sums of dw and db for
+// its columns over all the rows it walks; the CTAs write them as partial rows, and
+// a second launch adds those in CTA order: no atomics, the same bits on each run.
+//
+// Rows whose length is no multiple of a vector start at any element.  Their
+// vectors are those of the tensor: the first may begin in the row before, the last
+// ends where the row does.  What a row's start is off a vector's is the same for
+// all rows of a group, since the grid's stride is a multiple of its period.
+//
+// Rows longer than a CTA's registers hold, and tensors that do not start at 16
+// bytes, take the kernels that read a row more than once.
 #include <math.h>
 
+#include <algorithm>
+#include <type_traits>
+
+#include "f32x2.cuh"
 #include "rowvec.cuh"
 
 namespace tb {
@@ -24,98 +36,238 @@ namespace {
 
 using bf16 = __nv_bfloat16;
 
-// Columns a register kernel holds at most: 1024 threads of 8 elements.
-constexpr int64_t kLnMaxCols = 8192;
-// CTAs of the backward at most, so that the workspace is a function of the
-// shape: 1024 threads an SM on 148 SMs, in CTAs of 256 at least.
-constexpr int kLnSms = 148;
+constexpr int64_t kLnMaxCols = 8192;   // longer rows: the kernels of several passes
+constexpr int kLnStages = 3;           // rows in a ring, one of them being computed
+constexpr int kLnSms = 148;            // grids are functions of the shape alone, as the workspace is
 
-__device__ __forceinline__ float2 warp_sum2(float2 v) {
+__device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-        v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
-    }
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
 
-// Sum over a group of TPR threads; groups of more than a warp are the whole CTA
-// and go through `red` (TPR / 32 entries).  The caller alternates two buffers:
-// a thread that writes one again has passed the barrier of the other, which
+// Barrier of a group of NT consecutive threads, of R in the CTA.  A barrier whose number
+// is not a constant takes all 16 of a CTA, and four such CTAs all of an SM.
+template <int NT, int R>
+__device__ __forceinline__ void group_sync() {
+    if (R == 1) __syncthreads();
+    else asm volatile("bar.sync %0, %1;" ::"r"(1 + threadIdx.x / NT), "n"(NT) : "memory");
+}
+// Sums over a group; red has an entry for each of the CTA's warps.  The caller alternates
+// two of them: a thread that writes one again has passed the barrier of the other, which
 // every reader of the first has reached.
-template <int TPR>
-__device__ __forceinline__ float2 group_sum2(float2 v, float2* red) {
-    v = warp_sum2(v);
-    if (TPR == 32) return v;
-    constexpr int W = TPR / 32;
-    const int lane = threadIdx.x & 31;
-    if (lane == 0) red[threadIdx.x / 32] = v;
-    __syncthreads();
-    v = red[lane & (W - 1)];
+template <int NT, int R>
+__device__ __forceinline__ float group_sum(float v, float2* red) {
+    v = warp_sum(v);
+    if (NT == 32) return v;
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x / 32].x = v;
+    group_sync<NT, R>();
+    if (R > 1) red += threadIdx.x / NT * (NT / 32);
+    v = red[0].x;
 #pragma unroll
-    for (int o = W / 2; o > 0; o >>= 1) {
-        v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-        v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
-    }
+    for (int w = 1; w < NT / 32; w++) v += red[w].x;
     return v;
 }
-
-template <int TPR>
-__device__ __forceinline__ float group_sum(float v, float2* red) {
-    return group_sum2<TPR>(make_float2(v, 0.f), red).x;
+// Both sums in the shuffles of one and a half: the halves of the warp take one each.
+template <int NT, int R>
+__device__ __forceinline__ float2 group_sum2(float a, float b, float2* red) {
+    const bool high = threadIdx.x & 16;
+    float v = (high ? b : a) + __shfl_xor_sync(0xffffffffu, high ? a : b, 16);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    const float other = __shfl_xor_sync(0xffffffffu, v, 16);
+    float2 s = high ? make_float2(other, v) : make_float2(v, other);
+    if (NT == 32) return s;
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x / 32] = s;
+    group_sync<NT, R>();
+    if (R > 1) red += threadIdx.x / NT * (NT / 32);
+    s = red[0];
+#pragma unroll
+    for (int w = 1; w < NT / 32; w++) {
+        const float2 r = red[w];
+        s.x += r.x;
+        s.y += r.y;
+    }
+    return s;
 }
 
-// ---------------------------------------------------------------- forward --
-template <typename T, int V, int TPR, int EPT>
-__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) ln_fwd_kernel(const T* __restrict__ x, const T* __restrict__ w,
-                                                                       const T* __restrict__ b, T* __restrict__ y,
-                                                                       float* __restrict__ mean, float* __restrict__ rstd,
-                                                                       int64_t M, int N, float eps) {
-    constexpr int VPT = EPT / V, R = TPR == 32 ? 8 : 1;
-    __shared__ float2 red[2][TPR / 32];
-    const int t = threadIdx.x % TPR;
-    RowVec<T, V> wv[VPT], bv[VPT], xv[VPT];
-#pragma unroll
-    for (int i = 0; i < VPT; i++) {
-        const int c = (i * TPR + t) * V;
-        if (c < N) {
-            wv[i].load(w + c);
-            bv[i].load(b + c);
-        }
+// src_bytes of 16 from global memory, zeros behind them.
+__device__ __forceinline__ void copy16(uint4* smem, const void* global, int src_bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(smem)), "l"(global), "r"(src_bytes) : "memory");
+}
+__device__ __forceinline__ void copy4(float* smem, const float* global) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(smem)), "l"(global) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// A thread's columns of the rows of its group: VPT vectors of V, NT vectors apart.
+// SHIFT: rows may start inside a vector.
+template <typename T, int VPT, int NT, bool SHIFT>
+struct Cols {
+    static constexpr int V = 16 / sizeof(T), P = V / 2;
+    int c0, N;   // first column of the first vector; under 0 where it begins in the row before
+    // off: elements from a vector's start to the row's
+    __device__ __forceinline__ Cols(int N_, int off, int t) : c0(t * V - off), N(N_) {}
+    __device__ __forceinline__ int col(int i) const { return c0 + i * NT * V; }
+    __device__ __forceinline__ bool any(int i) const { return col(i) < N; }
+    __device__ __forceinline__ bool part(int i) const { return SHIFT && (col(i) < 0 || col(i) + V > N); }
+    __device__ __forceinline__ bool has(int i, int j) const { return (!SHIFT || col(i) + j >= 0) && col(i) + j < N; }
+    // a row's vector i into a slot; row points at column c0
+    __device__ __forceinline__ void copy(uint4* slot, const T* row, int i) const {
+        if (any(i)) copy16(slot, row + i * NT * V, SHIFT && col(i) + V > N ? (N - col(i)) * (int)sizeof(T) : 16);
     }
-    const float inv = 1.f / (float)N;
-    for (int64_t row = (int64_t)blockIdx.x * R + threadIdx.x / TPR; row < M; row += (int64_t)gridDim.x * R) {
-        const T* xr = x + row * N;
-        float s = 0.f;
+    // what is not the row's as 0; a branch of its own, as few warps have such a vector
+    __device__ __forceinline__ void mask(int i, F2* v) const {
+        if (part(i)) {
+            asm volatile("" ::: "memory");
 #pragma unroll
-        for (int i = 0; i < VPT; i++) {
-            const int c = (i * TPR + t) * V;
-            if (c < N) xv[i].load(xr + c);
-            else xv[i].zero();
-#pragma unroll
-            for (int j = 0; j < V; j++) s += xv[i].get(j);
-        }
-        const float mu = group_sum<TPR>(s, red[0]) * inv;
-        float q = 0.f;
-#pragma unroll
-        for (int i = 0; i < VPT; i++)
-            if ((i * TPR + t) * V < N)
-#pragma unroll
-                for (int j = 0; j < V; j++) {
-                    const float d = xv[i].get(j) - mu;
-                    q += d * d;
-                }
-        const float rs = rsqrtf(group_sum<TPR>(q, red[1]) * inv + eps);
-#pragma unroll
-        for (int i = 0; i < VPT; i++) {
-            const int c = (i * TPR + t) * V;
-            if (c < N) {
-                float o[V];
-#pragma unroll
-                for (int j = 0; j < V; j++) o[j] = (xv[i].get(j) - mu) * rs * wv[i].get(j) + bv[i].get(j);
-                RowVec<T, V>::store(y + row * N + c, o);
+            for (int j = 0; j < P; j++) {
+                float e[2];
+                get(v[j], e);
+                v[j] = f2(has(i, 2 * j) ? e[0] : 0.f, has(i, 2 * j + 1) ? e[1] : 0.f);
             }
         }
+    }
+    // zeros in the slots of vectors that no row has
+    __device__ __forceinline__ void clear(uint4* slot, int i) const {
+        if (!any(i)) *slot = make_uint4(0, 0, 0, 0);
+    }
+    // the slot's values, as pairs
+    __device__ __forceinline__ void load(const uint4* slot, int i, F2* v) const {
+        RowVec<T, V> r;
+        r.load(reinterpret_cast<const T*>(slot));
+#pragma unroll
+        for (int j = 0; j < P; j++) v[j] = f2(r.get(2 * j), r.get(2 * j + 1));
+        mask(i, v);
+    }
+    __device__ __forceinline__ void store(T* row, int i, const F2* v) const {
+        float e[V];
+#pragma unroll
+        for (int j = 0; j < P; j++) get(v[j], e + 2 * j);
+        if (part(i)) {
+#pragma unroll
+            for (int j = 0; j < V; j++)
+                if (has(i, j)) RowVec<T, 1>::store(row + i * NT * V + j, e + j);
+        } else if (any(i)) {
+            RowVec<T, V>::store(row + i * NT * V, e);
+        }
+    }
+    // a parameter (w, b) once, at any address
+    __device__ __forceinline__ void load_param(const T* p, F2* v) const {
+        if (!SHIFT && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+#pragma unroll
+            for (int i = 0; i < VPT; i++) {
+                RowVec<T, V> a;
+                a.zero();
+                if (any(i)) a.load(p + col(i));
+#pragma unroll
+                for (int j = 0; j < P; j++) v[i * P + j] = f2(a.get(2 * j), a.get(2 * j + 1));
+            }
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < VPT; i++)
+#pragma unroll
+            for (int j = 0; j < P; j++) {
+                RowVec<T, 1> a, b;
+                a.zero();
+                b.zero();
+                if (has(i, 2 * j)) a.load(p + col(i) + 2 * j);
+                if (has(i, 2 * j + 1)) b.load(p + col(i) + 2 * j + 1);
+                v[i * P + j] = f2(a.get(0), b.get(0));
+            }
+    }
+};
+
+// Elements from the last vector's start to row m's.
+template <typename T>
+__device__ __forceinline__ int row_offset(int64_t m, int N) {
+    return (int)((uint64_t)m * (uint64_t)N % (16 / sizeof(T)));
+}
+
+// Threads of a CTA: the forward's groups are CTAs of their own (warps go eight to one), the
+// backward's share one as large as registers allow, whose groups add their sums of dw and db
+// in shared memory first.
+template <int NT>
+constexpr int fwd_cta() { return NT == 32 ? 256 : NT; }
+template <int NT>
+constexpr int bwd_cta() { return NT % 3 ? 512 : 384; }
+
+// ---------------------------------------------------------------- forward --
+template <typename T, int VPT, int NT, bool SHIFT>
+__global__ void __launch_bounds__(fwd_cta<NT>()) ln_fwd_kernel(const T* __restrict__ x, const T* __restrict__ w,
+                                                              const T* __restrict__ b, T* __restrict__ y,
+                                                              float* __restrict__ mean, float* __restrict__ rstd, int64_t M,
+                                                              int N, float eps) {
+    using C = Cols<T, VPT, NT, SHIFT>;
+    constexpr int P = C::P, K = P * VPT, S = kLnStages, CTA = fwd_cta<NT>(), R = CTA / NT;
+    extern __shared__ uint4 ring[];   // [S][VPT][CTA]
+    __shared__ float2 red[2][CTA / 32];
+    const int t = threadIdx.x % NT;
+    const int64_t first = (int64_t)blockIdx.x * R + threadIdx.x / NT, stride = (int64_t)gridDim.x * R;
+    if (first >= M) return;   // the whole group
+    const C cols(N, SHIFT ? row_offset<T>(first, N) : 0, t);
+    const int64_t step = stride * N;
+    const T* xp = x + first * N + cols.c0;   // of the next row to fetch
+    T* yp = y + first * N + cols.c0;
+    int ahead = (int)((M - first + stride - 1) / stride);   // rows left to fetch
+    auto fetch = [&](uint4* slot) {
+        if (ahead-- > 0)
+#pragma unroll
+            for (int i = 0; i < VPT; i++) cols.copy(slot + i * CTA, xp, i);
+        copy_commit();
+        xp += step;
+    };
+    uint4* const base = ring + threadIdx.x;
+#pragma unroll
+    for (int s = 0; s < S * VPT; s++) cols.clear(base + s * CTA, s % VPT);
+#pragma unroll
+    for (int s = 0; s < S - 1; s++) fetch(base + s * VPT * CTA);
+    F2 wv[K], bv[K];
+    cols.load_param(w, wv);
+    cols.load_param(b, bv);
+    const float inv = 1.f / (float)N;
+    uint4 *slot = base, *last = base + (S - 1) * VPT * CTA;
+    for (int64_t row = first; row < M; row += stride) {
+        fetch(last);
+        copy_wait<S - 1>();
+        F2 v[K], sum = f2(0.f);
+        float e[2];
+#pragma unroll
+        for (int i = 0; i < VPT; i++) {
+            cols.load(slot + i * CTA, i, v + i * P);
+#pragma unroll
+            for (int j = 0; j < P; j++) sum = add(sum, v[i * P + j]);
+        }
+        last = slot;
+        slot = slot + VPT * CTA < base + S * VPT * CTA ? slot + VPT * CTA : base;
+        get(sum, e);
+        const float mu = group_sum<NT, R>(e[0] + e[1], red[0]) * inv;
+        const F2 minus = f2(-mu);
+        F2 q = f2(0.f);
+#pragma unroll
+        for (int i = 0; i < VPT; i++) {
+#pragma unroll
+            for (int j = 0; j < P; j++) v[i * P + j] = add(v[i * P + j], minus);
+            if (SHIFT) cols.mask(i, v + i * P);
+            if (cols.any(i))
+#pragma unroll
+                for (int j = 0; j < P; j++) q = fma(v[i * P + j], v[i * P + j], q);
+        }
+        get(q, e);
+        const float rs = rsqrtf(group_sum<NT, R>(e[0] + e[1], red[1]) * inv + eps);
+        const F2 rs2 = f2(rs);
+#pragma unroll
+        for (int i = 0; i < VPT; i++) {
+#pragma unroll
+            for (int j = 0; j < P; j++) v[i * P + j] = fma(mul(v[i * P + j], rs2), wv[i * P + j], bv[i * P + j]);
+            cols.store(yp, i, v + i * P);
+        }
+        yp += step;
         if (t == 0) {
             mean[row] = mu;
             rstd[row] = rs;
@@ -123,8 +275,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) ln_fwd_kernel(const T* 
     }
 }
 
-// Rows longer than kLnMaxCols: one CTA a row, three passes (the second and
-// third find the row in L2).
+// Any row: one CTA, three passes (the second and third find the row in L2).
 template <typename T, int V>
 __global__ void __launch_bounds__(1024) ln_fwd_wide_kernel(const T* __restrict__ x, const T* __restrict__ w,
                                                            const T* __restrict__ b, T* __restrict__ y,
@@ -141,7 +292,7 @@ __global__ void __launch_bounds__(1024) ln_fwd_wide_kernel(const T* __restrict__
 #pragma unroll
         for (int j = 0; j < V; j++) s += v.get(j);
     }
-    const float mu = group_sum<1024>(s, red[0]) * inv;
+    const float mu = group_sum<1024, 1>(s, red[0]) * inv;
     float q = 0.f;
     for (int64_t c = (int64_t)threadIdx.x * V; c < N; c += 1024 * V) {
         v.load(xr + c);
@@ -151,7 +302,7 @@ __global__ void __launch_bounds__(1024) ln_fwd_wide_kernel(const T* __restrict__
             q += d * d;
         }
     }
-    const float rs = rsqrtf(group_sum<1024>(q, red[1]) * inv + eps);
+    const float rs = rsqrtf(group_sum<1024, 1>(q, red[1]) * inv + eps);
     for (int64_t c = (int64_t)threadIdx.x * V; c < N; c += 1024 * V) {
         v.load(xr + c);
         g.load(w + c);
@@ -169,100 +320,119 @@ __global__ void __launch_bounds__(1024) ln_fwd_wide_kernel(const T* __restrict__
 
 // --------------------------------------------------------------- backward --
 // part: [gridDim.x][2][N], the CTA's sums of dw and db.
-template <typename T, int V, int TPR, int EPT>
-__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) ln_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x,
-                                                                       const T* __restrict__ w,
-                                                                       const float* __restrict__ mean,
-                                                                       const float* __restrict__ rstd, T* __restrict__ dx,
-                                                                       float* __restrict__ part, int64_t M, int N) {
-    constexpr int VPT = EPT / V, R = TPR == 32 ? 8 : 1;
-    __shared__ float2 red[2][TPR / 32];
-    const int t = threadIdx.x % TPR;
-    RowVec<T, V> wv[VPT], xv[VPT], gv[VPT];
-    float aw[EPT], ab[EPT];
+template <typename T, int VPT, int NT, bool SHIFT>
+__global__ void __launch_bounds__(bwd_cta<NT>()) ln_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x,
+                                                              const T* __restrict__ w, const float* __restrict__ mean,
+                                                              const float* __restrict__ rstd, T* __restrict__ dx,
+                                                              float* __restrict__ part, int64_t M, int N) {
+    using C = Cols<T, VPT, NT, SHIFT>;
+    constexpr int P = C::P, K = P * VPT, S = kLnStages, CTA = bwd_cta<NT>(), R = CTA / NT;
+    extern __shared__ uint4 ring[];   // [S][x, dy][VPT][CTA]
+    __shared__ float2 stats[S][CTA];  // each thread's copies of mean and rstd
+    __shared__ float2 red[2][CTA / 32];
+    const int t = threadIdx.x % NT;
+    const int64_t first = (int64_t)blockIdx.x * R + threadIdx.x / NT, stride = (int64_t)gridDim.x * R;
+    const C cols(N, SHIFT ? row_offset<T>(first, N) : 0, t);
+    const int64_t step = stride * N;
+    const T *xp = x + first * N + cols.c0, *gp = dy + first * N + cols.c0;   // of the next row to fetch
+    T* op = dx + first * N + cols.c0;
+    int left = first < M ? (int)((M - first + stride - 1) / stride) : 0, ahead = left;   // rows; rows to fetch
+    const float *mp = mean + first, *rp = rstd + first;
+    auto fetch = [&](int s) {
+        if (ahead-- > 0) {
+            uint4* slot = ring + s * 2 * VPT * CTA + threadIdx.x;
 #pragma unroll
-    for (int i = 0; i < VPT; i++) {
-        const int c = (i * TPR + t) * V;
-        if (c < N) wv[i].load(w + c);
-        else wv[i].zero();
+            for (int i = 0; i < VPT; i++) {
+                cols.copy(slot + i * CTA, xp, i);
+                cols.copy(slot + (VPT + i) * CTA, gp, i);
+            }
+            copy4(&stats[s][threadIdx.x].x, mp);
+            copy4(&stats[s][threadIdx.x].y, rp);
+        }
+        copy_commit();
+        xp += step;
+        gp += step;
+        mp += stride;
+        rp += stride;
+    };
 #pragma unroll
-        for (int j = 0; j < V; j++) aw[i * V + j] = ab[i * V + j] = 0.f;
-    }
+    for (int s = 0; s < S * 2 * VPT; s++) cols.clear(ring + s * CTA + threadIdx.x, s % VPT);
+#pragma unroll
+    for (int s = 0; s < S - 1; s++) fetch(s);
+    F2 wv[K], aw[K], ab[K];
+    cols.load_param(w, wv);
+#pragma unroll
+    for (int k = 0; k < K; k++) aw[k] = ab[k] = f2(0.f);
     const float inv = 1.f / (float)N;
-    int buf = 0;
-    for (int64_t row = (int64_t)blockIdx.x * R + threadIdx.x / TPR; row < M; row += (int64_t)gridDim.x * R) {
-        const float mu = mean[row], rs = rstd[row];
+    int s = 0, buf = 0;
+    for (; left > 0; left--) {
+        fetch(s ? s - 1 : S - 1);
+        copy_wait<S - 1>();
+        const uint4* slot = ring + s * 2 * VPT * CTA + threadIdx.x;
+        const float mu = stats[s][threadIdx.x].x, rs = stats[s][threadIdx.x].y;
+        F2 xh[K], a[K], sa = f2(0.f), sx = f2(0.f);
+        const F2 minus = f2(-mu), r = f2(rs);
 #pragma unroll
         for (int i = 0; i < VPT; i++) {
-            const int c = (i * TPR + t) * V;
-            if (c < N) {
-                xv[i].load(x + row * N + c);
-                gv[i].load(dy + row * N + c);
-            } else {
-                xv[i].zero();
-                gv[i].zero();
+            cols.load(slot + i * CTA, i, xh + i * P);
+            cols.load(slot + (VPT + i) * CTA, i, a + i * P);
+#pragma unroll
+            for (int k = i * P; k < i * P + P; k++) {
+                xh[k] = mul(add(xh[k], minus), r);
+                aw[k] = fma(a[k], xh[k], aw[k]);
+                ab[k] = add(ab[k], a[k]);
+                a[k] = mul(a[k], wv[k]);
+                sa = add(sa, a[k]);
+                sx = fma(a[k], xh[k], sx);
             }
         }
-        float2 s = make_float2(0.f, 0.f);
-#pragma unroll
-        for (int i = 0; i < VPT; i++)
-#pragma unroll
-            for (int j = 0; j < V; j++) {
-                const float g = gv[i].get(j), xh = (xv[i].get(j) - mu) * rs, a = g * wv[i].get(j);
-                s.x += a;
-                s.y += a * xh;
-                aw[i * V + j] += g * xh;
-                ab[i * V + j] += g;
-            }
-        s = group_sum2<TPR>(s, red[buf]);
+        s = s + 1 < S ? s + 1 : 0;
+        float e[2], f[2];
+        get(sa, e);
+        get(sx, f);
+        const float2 sum = group_sum2<NT, R>(e[0] + e[1], f[0] + f[1], red[buf]);
         buf ^= 1;
-        const float c1 = s.x * inv, c2 = s.y * inv;
+        const F2 k1 = f2(-sum.x * inv * rs), k2 = f2(-sum.y * inv * rs);
 #pragma unroll
         for (int i = 0; i < VPT; i++) {
-            const int c = (i * TPR + t) * V;
-            if (c < N) {
-                float o[V];
 #pragma unroll
-                for (int j = 0; j < V; j++) {
-                    const float xh = (xv[i].get(j) - mu) * rs;
-                    o[j] = rs * (gv[i].get(j) * wv[i].get(j) - c1 - xh * c2);
-                }
-                RowVec<T, V>::store(dx + row * N + c, o);
-            }
+            for (int k = i * P; k < i * P + P; k++) a[k] = fma(xh[k], k2, fma(a[k], r, k1));
+            cols.store(op, i, a + i * P);
         }
+        op += step;
     }
-    if (R > 1) {   // the warps' sums, added in warp order
-        __shared__ float sw[R > 1 ? 32 * EPT : 1], sb[R > 1 ? 32 * EPT : 1];
-        for (int r = 0; r < R; r++) {
-            if (threadIdx.x / 32 == r)
-#pragma unroll
-                for (int k = 0; k < EPT; k++) {
-                    const int c = k * 32 + t;
-                    if (r) {
-                        aw[k] += sw[c];
-                        ab[k] += sb[c];
-                    }
-                    sw[c] = aw[k];
-                    sb[c] = ab[k];
-                }
-            __syncthreads();
-        }
-        if (threadIdx.x / 32 != R - 1) return;
-    }
-    float* pw = part + (int64_t)blockIdx.x * 2 * N;
+    // The groups' sums to shared memory, where the rings were, and from there added in their order.  Their
+    // columns differ where their rows' offsets do.
+    pdl_trigger();
+    float* sw = reinterpret_cast<float*>(ring);   // [R][2][N]
+    copy_wait<0>();
+    __syncthreads();
+    float* mine = sw + threadIdx.x / NT * 2 * N;
 #pragma unroll
     for (int i = 0; i < VPT; i++)
 #pragma unroll
-        for (int j = 0; j < V; j++) {
-            const int c = (i * TPR + t) * V + j;
-            if (c < N) {
-                pw[c] = aw[i * V + j];
-                pw[N + c] = ab[i * V + j];
-            }
+        for (int j = 0; j < P; j++) {
+            float e[2], f[2];
+            get(aw[i * P + j], e);
+            get(ab[i * P + j], f);
+#pragma unroll
+            for (int o = 0; o < 2; o++)
+                if (cols.has(i, 2 * j + o)) {
+                    mine[cols.col(i) + 2 * j + o] = e[o];
+                    mine[N + cols.col(i) + 2 * j + o] = f[o];
+                }
         }
+    __syncthreads();
+    float* pw = part + (int64_t)blockIdx.x * 2 * N;
+    for (int c = threadIdx.x; c < 2 * N; c += CTA) {
+        float v = sw[c];
+#pragma unroll
+        for (int g = 1; g < R; g++) v += sw[g * 2 * N + c];
+        pw[c] = v;
+    }
 }
 
-// Long rows: dx by one CTA a row, two passes.
+// Any row: dx by one CTA, two passes.
 template <typename T, int V>
 __global__ void __launch_bounds__(1024) ln_bwd_wide_dx_kernel(const T* __restrict__ dy, const T* __restrict__ x,
                                                               const T* __restrict__ w, const float* __restrict__ mean,
@@ -284,7 +454,7 @@ __global__ void __launch_bounds__(1024) ln_bwd_wide_dx_kernel(const T* __restric
             s.y += a * ((xv.get(j) - mu) * rs);
         }
     }
-    s = group_sum2<1024>(s, red);
+    s = group_sum2<1024, 1>(s.x, s.y, red);
     const float c1 = s.x * inv, c2 = s.y * inv;
     for (int64_t c = (int64_t)threadIdx.x * V; c < N; c += 1024 * V) {
         xv.load(x + base + c);
@@ -298,7 +468,7 @@ __global__ void __launch_bounds__(1024) ln_bwd_wide_dx_kernel(const T* __restric
     }
 }
 
-// Long rows: dw and db over the rows of split blockIdx.y, V columns a thread.
+// Any rows: dw and db over the rows of split blockIdx.y, V columns a thread.
 template <typename T, int V>
 __global__ void __launch_bounds__(256) ln_bwd_wide_cols_kernel(const T* __restrict__ dy, const T* __restrict__ x,
                                                                const float* __restrict__ mean,
@@ -331,90 +501,156 @@ __global__ void __launch_bounds__(256) ln_bwd_wide_cols_kernel(const T* __restri
 }
 
 // dw[n] (+)= sum_g part[g][0][n], db[n] (+)= sum_g part[g][1][n].  32 columns by
-// 16 lanes of rows a CTA; the lanes' sums are added in lane order.
-__global__ void __launch_bounds__(512) ln_bwd_final_kernel(const float* __restrict__ part, float* __restrict__ dw,
-                                                           float* __restrict__ db, int64_t N, int G, int accumulate) {
-    __shared__ float red[16][33];
+// 32 lanes of rows a CTA, a lane's loads (5 for 148 rows) in flight together; the
+// lanes' sums are added in a fixed tree.
+__global__ void __launch_bounds__(1024) ln_bwd_final_kernel(const float* __restrict__ part, float* __restrict__ dw,
+                                                            float* __restrict__ db, int64_t N, int G, int accumulate) {
+    __shared__ float red[32][33];
+    pdl_wait();
     const int64_t c = (int64_t)blockIdx.x * 32 + threadIdx.x;
     float s = 0.f;
     if (c < 2 * N)
-#pragma unroll 4
-        for (int g = threadIdx.y; g < G; g += 16) s += part[(int64_t)g * 2 * N + c];
+        for (int g0 = threadIdx.y; g0 < G; g0 += 32 * 5) {
+            float v[5];
+#pragma unroll
+            for (int k = 0; k < 5; k++) v[k] = g0 + 32 * k < G ? part[(int64_t)(g0 + 32 * k) * 2 * N + c] : 0.f;
+#pragma unroll
+            for (int k = 0; k < 5; k++) s += v[k];
+        }
     red[threadIdx.y][threadIdx.x] = s;
     __syncthreads();
-    if (threadIdx.y || c >= 2 * N) return;
-#pragma unroll
-    for (int k = 1; k < 16; k++) s += red[k][threadIdx.x];
-    float* out = c < N ? dw + c : db + (c - N);
+    s = warp_sum(red[threadIdx.x][threadIdx.y]);   // the warp of column threadIdx.y
+    const int64_t col = (int64_t)blockIdx.x * 32 + threadIdx.y;
+    if (threadIdx.x || col >= 2 * N) return;
+    float* out = col < N ? dw + col : db + (col - N);
     *out = accumulate ? *out + s : s;
 }
 
 // ------------------------------------------------------------------- host --
-// Threads that share a row, and the rows a CTA takes at a time.
-int group_threads(int64_t N) { return N <= 256 ? 32 : N <= 1024 ? 128 : N <= 2048 ? 256 : N <= 4096 ? 512 : 1024; }
-
-// Rows of partial sums that the backward writes.
-int64_t bwd_parts(int64_t M, int64_t N) {
-    if (N > kLnMaxCols) {
-        // two CTAs an SM or so over tiles of at most 2048 columns, 16 rows a split at least
-        const int64_t tiles = (N + 2047) / 2048, want = (2 * kLnSms + tiles - 1) / tiles, most = (M + 15) / 16;
-        return want < most ? want : most;
-    }
-    const int tpr = group_threads(N), threads = tpr == 32 ? 256 : tpr, rows = tpr == 32 ? 8 : 1;
-    const int64_t want = (int64_t)kLnSms * (1024 / threads), most = (M + rows - 1) / rows;
-    return want < most ? want : most;
+// Threads of a row's group: 16 elements each, a warp up to 512 elements.
+int group_of(int64_t N, int esz) {
+    const int V = 16 / esz;
+    const int64_t most = N + (N % V ? V - 1 : 0);   // with the largest offset
+    for (int threads : {32, 64, 128, 192, 256, 384})
+        if (most <= threads * 16) return threads;
+    return 512;
 }
 
-template <typename T, int V>
+// Whether the one-pass kernels take a shape (their tensors at 16 bytes).
+bool one_pass(int64_t N, int esz) {
+    const int V = 16 / esz;
+    return N + (N % V ? V - 1 : 0) <= kLnMaxCols;
+}
+
+// CTAs for M rows, `rows` of them a CTA at a time and `ctas` to an SM: a number whose stride keeps the rows' offsets
+// (their period divides V), or one for each row.
+int64_t ctas_for(int64_t M, int64_t N, int esz, int rows, int ctas) {
+    const int V = 16 / esz;
+    int64_t want = (int64_t)kLnSms * ctas;
+    while (N % V && want * rows % V) want--;
+    return std::min(want, (M + rows - 1) / rows);
+}
+// 768 threads an SM, 1024 where a CTA has 512: fewer leave HBM idle, more wait for shared memory and for one another
+// (16384 x 2048 bf16 with 512 / 768 / 1024 / 1536: 24.4 / 22.1 / 25.6 / 24.1 us; 4096 x 8192 f32: 62 / 62 / 50 / 60).
+int fwd_ctas(int threads) { return (threads == 512 ? 1024 : 768) / threads; }
+int64_t bwd_ctas(int64_t M, int64_t N, int esz) {
+    const int nt = group_of(N, esz);
+    return ctas_for(M, N, esz, (nt % 3 ? 512 : 384) / nt, 1);
+}
+
+// Rows of partial sums that the several-pass backward writes: two CTAs an SM or so over tiles of 256 columns at
+// least, 16 rows a split at least.
+int64_t wide_parts(int64_t M, int64_t N) {
+    const int64_t tiles = (N + 2047) / 2048;
+    return std::max<int64_t>(1, std::min((2 * kLnSms + tiles - 1) / tiles, (M + 15) / 16));
+}
+
+template <typename T>
 int fwd(tb_ctx* ctx, const T* x, const T* w, const T* b, T* y, float* mean, float* rstd, int64_t M, int64_t N, float eps) {
-    if (N > kLnMaxCols)
-        return launch(ctx, "layernorm_fwd_wide", ln_fwd_wide_kernel<T, V>, dim3((unsigned)M), dim3(1024), 0, x, w, b, y,
-                      mean, rstd, N, eps);
-    const int tpr = group_threads(N), threads = tpr == 32 ? 256 : tpr, rows = tpr == 32 ? 8 : 1;
-    const int64_t want = (int64_t)ctx->num_sms * (2048 / threads), most = (M + rows - 1) / rows;
-    const dim3 grid((unsigned)(want < most ? want : most));
-    auto go = [&](auto kern) {
-        return launch(ctx, "layernorm_fwd", kern, grid, dim3(threads), 0, x, w, b, y, mean, rstd, M, (int)N, eps);
-    };
-    switch (tpr) {
-        case 32: return go(ln_fwd_kernel<T, V, 32, 8>);
-        case 128: return go(ln_fwd_kernel<T, V, 128, 8>);
-        case 256: return go(ln_fwd_kernel<T, V, 256, 8>);
-        case 512: return go(ln_fwd_kernel<T, V, 512, 8>);
-        default: return go(ln_fwd_kernel<T, V, 1024, 8>);
+    constexpr int V = 16 / sizeof(T);
+    if (!one_pass(N, sizeof(T)) || !aligned16(x) || !aligned16(y)) {
+        const bool vec = N % V == 0 && aligned16(x) && aligned16(y) && aligned16(w) && aligned16(b);
+        return launch(ctx, "layernorm_fwd_wide", vec ? ln_fwd_wide_kernel<T, V> : ln_fwd_wide_kernel<T, 1>, dim3((unsigned)M),
+                      dim3(1024), 0, x, w, b, y, mean, rstd, N, eps);
     }
+    const int nt = group_of(N, sizeof(T)), threads = nt == 32 ? 256 : nt;
+    const int64_t grid = ctas_for(M, N, sizeof(T), threads / nt, fwd_ctas(threads));
+    const int smem = kLnStages * threads * 16 * (int)sizeof(T);
+    auto go = [&](auto kern) {
+        if (smem > 47 * 1024)   // with the static part, past what a kernel has unasked
+            TB_CUDA_TRY(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        return launch(ctx, "layernorm_fwd", kern, dim3((unsigned)grid), dim3(threads), smem, x, w, b, y, mean, rstd, M,
+                      (int)N, eps);
+    };
+    auto of = [&](auto shift) {
+        constexpr bool SH = decltype(shift)::value;
+        constexpr int K = 16 / V;
+        switch (nt) {
+            case 32: return go(ln_fwd_kernel<T, K, 32, SH>);
+            case 64: return go(ln_fwd_kernel<T, K, 64, SH>);
+            case 128: return go(ln_fwd_kernel<T, K, 128, SH>);
+            case 192: return go(ln_fwd_kernel<T, K, 192, SH>);
+            case 256: return go(ln_fwd_kernel<T, K, 256, SH>);
+            case 384: return go(ln_fwd_kernel<T, K, 384, SH>);
+            default: return go(ln_fwd_kernel<T, K, 512, SH>);
+        }
+    };
+    return N % V ? of(std::true_type()) : of(std::false_type());
 }
 
-template <typename T, int V>
+template <typename T>
 int bwd(tb_ctx* ctx, const T* dy, const T* x, const T* w, const float* mean, const float* rstd, T* dx, float* dw, float* db,
         int accumulate, int64_t M, int64_t N, float* part) {
-    const int64_t G = bwd_parts(M, N);
+    constexpr int V = 16 / sizeof(T);
+    int64_t G;
     int rc;
-    if (N > kLnMaxCols) {
-        rc = launch(ctx, "layernorm_bwd_wide", ln_bwd_wide_dx_kernel<T, V>, dim3((unsigned)M), dim3(1024), 0, dy, x, w,
-                    mean, rstd, dx, N);
+    if (!one_pass(N, sizeof(T)) || !aligned16(x) || !aligned16(dy) || !aligned16(dx)) {
+        const bool vec = N % V == 0 && aligned16(x) && aligned16(dy) && aligned16(dx) && aligned16(w);
+        const int cols = 256 * (vec ? V : 1);
+        G = wide_parts(M, N);
+        rc = launch(ctx, "layernorm_bwd_wide", vec ? ln_bwd_wide_dx_kernel<T, V> : ln_bwd_wide_dx_kernel<T, 1>,
+                    dim3((unsigned)M), dim3(1024), 0, dy, x, w, mean, rstd, dx, N);
         if (rc) return rc;
-        const int64_t rows = (M + G - 1) / G;
-        rc = launch(ctx, "layernorm_bwd_cols", ln_bwd_wide_cols_kernel<T, V>,
-                    dim3((unsigned)((N + 256 * V - 1) / (256 * V)), (unsigned)G), dim3(256), 0, dy, x, mean, rstd, part, M,
-                    N, rows);
+        rc = launch(ctx, "layernorm_bwd_cols", vec ? ln_bwd_wide_cols_kernel<T, V> : ln_bwd_wide_cols_kernel<T, 1>,
+                    dim3((unsigned)((N + cols - 1) / cols), (unsigned)G), dim3(256), 0, dy, x, mean, rstd, part, M, N,
+                    (M + G - 1) / G);
     } else {
-        const int tpr = group_threads(N), threads = tpr == 32 ? 256 : tpr;
+        const int nt = group_of(N, sizeof(T)), threads = nt % 3 ? 512 : 384;
+        G = bwd_ctas(M, N, sizeof(T));
+        const int smem = kLnStages * 2 * threads * 16 * (int)sizeof(T);   // the groups' sums take 8 N bytes each, 64 KB at most
         auto go = [&](auto kern) {
-            return launch(ctx, "layernorm_bwd", kern, dim3((unsigned)G), dim3(threads), 0, dy, x, w, mean, rstd, dx, part, M,
-                          (int)N);
+            TB_CUDA_TRY(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+            return launch(ctx, "layernorm_bwd", kern, dim3((unsigned)G), dim3(threads), smem, dy, x, w, mean, rstd, dx, part,
+                          M, (int)N);
         };
-        switch (tpr) {
-            case 32: rc = go(ln_bwd_kernel<T, V, 32, 8>); break;
-            case 128: rc = go(ln_bwd_kernel<T, V, 128, 8>); break;
-            case 256: rc = go(ln_bwd_kernel<T, V, 256, 8>); break;
-            case 512: rc = go(ln_bwd_kernel<T, V, 512, 8>); break;
-            default: rc = go(ln_bwd_kernel<T, V, 1024, 8>); break;
-        }
+        auto of = [&](auto shift) {
+            constexpr bool SH = decltype(shift)::value;
+            constexpr int K = 16 / V;
+            switch (nt) {
+                case 32: return go(ln_bwd_kernel<T, K, 32, SH>);
+                case 64: return go(ln_bwd_kernel<T, K, 64, SH>);
+                case 128: return go(ln_bwd_kernel<T, K, 128, SH>);
+                case 192: return go(ln_bwd_kernel<T, K, 192, SH>);
+                case 256: return go(ln_bwd_kernel<T, K, 256, SH>);
+                case 384: return go(ln_bwd_kernel<T, K, 384, SH>);
+                default: return go(ln_bwd_kernel<T, K, 512, SH>);
+            }
+        };
+        rc = N % V ? of(std::true_type()) : of(std::false_type());
     }
     if (rc) return rc;
-    return launch(ctx, "layernorm_bwd_final", ln_bwd_final_kernel, dim3((unsigned)((2 * N + 31) / 32)), dim3(32, 16), 0,
-                  (const float*)part, dw, db, N, (int)G, accumulate);
+    // launched while the last CTAs still run: it waits for them itself
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = dim3((unsigned)((2 * N + 31) / 32));
+    lc.blockDim = dim3(32, 32);
+    lc.stream = ctx->stream;
+    cudaLaunchAttribute early[1];
+    early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early[0].val.programmaticStreamSerializationAllowed = 1;
+    lc.attrs = early;
+    lc.numAttrs = 1;
+    TB_CUDA_TRY(ctx, cudaLaunchKernelEx(&lc, ln_bwd_final_kernel, (const float*)part, dw, db, N, (int)G, accumulate));
+    return TB_OK;
 }
 
 // Whether the bytes at p meet those at q.
@@ -446,13 +682,9 @@ int tb_layernorm_fwd_train(tb_ctx* ctx, int dtype, const void* x, const void* w,
     const size_t es = dtype == TB_F32 ? 4 : 2, row = es * (size_t)N, all = row * (size_t)M;
     TB_REQUIRE(ctx, !meet(y, all, x, all) && !meet(y, all, w, row) && !meet(y, all, b, row), TB_ERR_ARG,
                "layernorm_fwd_train: y overlaps an input");
-    const bool vec = aligned16(x) && aligned16(w) && aligned16(b) && aligned16(y);
-    if (dtype == TB_F32) {
-        auto f = vec && N % 4 == 0 ? fwd<float, 4> : fwd<float, 1>;
-        return f(ctx, (const float*)x, (const float*)w, (const float*)b, (float*)y, mean, rstd, M, N, eps);
-    }
-    auto f = vec && N % 8 == 0 ? fwd<bf16, 8> : fwd<bf16, 1>;
-    return f(ctx, (const bf16*)x, (const bf16*)w, (const bf16*)b, (bf16*)y, mean, rstd, M, N, eps);
+    if (dtype == TB_F32)
+        return fwd(ctx, (const float*)x, (const float*)w, (const float*)b, (float*)y, mean, rstd, M, N, eps);
+    return fwd(ctx, (const bf16*)x, (const bf16*)w, (const bf16*)b, (bf16*)y, mean, rstd, M, N, eps);
 }
 
 int tb_layernorm_bwd(tb_ctx* ctx, int dtype, const void* dy, const void* x, const void* w, const float* mean,
@@ -478,18 +710,19 @@ int tb_layernorm_bwd(tb_ctx* ctx, int dtype, const void* dy, const void* x, cons
     TB_REQUIRE(ctx, !meet(dx, all, x, all) && !meet(dx, all, dy, all) && !meet(dx, all, w, row) && !meet(dw, sums, db, sums),
                TB_ERR_ARG, "layernorm_bwd: an output overlaps another tensor");
     float* part = reinterpret_cast<float*>(workspace);
-    const bool vec = aligned16(dy) && aligned16(x) && aligned16(w) && aligned16(dx);
-    if (dtype == TB_F32) {
-        auto f = vec && N % 4 == 0 ? bwd<float, 4> : bwd<float, 1>;
-        return f(ctx, (const float*)dy, (const float*)x, (const float*)w, mean, rstd, (float*)dx, dw, db, accumulate, M, N,
-                 part);
-    }
-    auto f = vec && N % 8 == 0 ? bwd<bf16, 8> : bwd<bf16, 1>;
-    return f(ctx, (const bf16*)dy, (const bf16*)x, (const bf16*)w, mean, rstd, (bf16*)dx, dw, db, accumulate, M, N, part);
+    if (dtype == TB_F32)
+        return bwd(ctx, (const float*)dy, (const float*)x, (const float*)w, mean, rstd, (float*)dx, dw, db, accumulate, M, N,
+                   part);
+    return bwd(ctx, (const bf16*)dy, (const bf16*)x, (const bf16*)w, mean, rstd, (bf16*)dx, dw, db, accumulate, M, N, part);
 }
 
 size_t tb_layernorm_bwd_ws(int64_t M, int64_t N) {
-    return ln_shape_ok(M, N) ? (size_t)bwd_parts(M, N) * 2 * (size_t)N * 4 : 0;
+    if (!ln_shape_ok(M, N) || !M) return 0;
+    // enough for either type and either kernel
+    int64_t parts = wide_parts(M, N);
+    for (int esz = 2; esz <= 4; esz += 2)
+        if (one_pass(N, esz)) parts = std::max(parts, bwd_ctas(M, N, esz));
+    return (size_t)parts * 2 * (size_t)N * 4;
 }
 
 }  // extern "C"

@@ -22,8 +22,7 @@
 //    probability of the rest, by 16 bits each of a hash of (seed, step, tensor,
 //    element): the mean over the steps is the 32-bit moment's, and a run repeats.
 //  * Each operation up to the code is rounded by itself (no fused multiply-add),
-//    so the codes are defined bit for bit by the formula, but for the last place
-//    of the square root.
+//    so the codes are defined bit for bit by the formula.
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <math.h>
@@ -33,6 +32,7 @@
 #include <new>
 
 #include "common.cuh"
+#include "f32x2.cuh"
 
 namespace tb {
 namespace {
@@ -254,26 +254,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) adamw_kernel(const __gri
     }
 }
 
-// Two f32 in one instruction, each rounded as by itself.
-struct F2 {
-    unsigned long long v;
-};
-__device__ __forceinline__ F2 f2(float a, float b) {
-    F2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void get(F2 a, float* v) { asm("mov.b64 {%0, %1}, %2;" : "=f"(v[0]), "=f"(v[1]) : "l"(a.v)); }
-__device__ __forceinline__ F2 mul(F2 a, F2 b) {
-    F2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-    return r;
-}
-__device__ __forceinline__ F2 fma(F2 a, F2 b, F2 c) {
-    F2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-    return r;
-}
 // Two sums.  Packed, they were contracted with the products they add; scalar ones with a rounding of their own are not.
 __device__ __forceinline__ void sums(F2 a, F2 b, float* v) {
     float x[2], y[2];
@@ -431,7 +411,8 @@ __device__ __forceinline__ void fetch(UnitIn<P, G>& in, const Entry& e, int unit
 
 // The two blocks of a whole unit at aligned addresses; false, with nothing written, where one is
 // not a common one.  The common case folds the exponents into the betas (exact, as they are powers
-// of two) and takes the hardware's square root (2^-23), which flushes what is under 2^-126.
+// of two) and takes the hardware's square root (2^-23), which flushes what is under 2^-126, where
+// no code depends on its last places.
 // exps: m's exponents in bytes 0 and 1, s's in 2 and 3.
 template <typename P, typename G>
 __device__ __forceinline__ bool adamw8_unit(const UnitIn<P, G>& in, uint32_t exps, const Entry& e, int unit, const Hyper& h,
@@ -492,7 +473,7 @@ __device__ __forceinline__ bool adamw8_unit(const UnitIn<P, G>& in, uint32_t exp
         for (int u = 0; u < 2; u++) {
             const int o = b * kBlock + u * 128;
             float p[4];
-            uint32_t wm[4], ws[4];
+            uint32_t wm[4], ws[4], border = ~0u;
             load4(in.p + o + at, p);
 #pragma unroll
             for (int j = 0; j < 4; j += 2) {
@@ -510,9 +491,20 @@ __device__ __forceinline__ bool adamw8_unit(const UnitIn<P, G>& in, uint32_t exp
                     // 16 x + r: the code's bits 20 to 26 come to 24 to 30, and the sign goes back to 31
                     wm[j + w] = (__float_as_uint(x[w]) * 16u + rm) | (__float_as_uint(x[w]) & 0x80000000u);
                     ws[j + w] = __float_as_uint(y[w]) * 16u + rs;
-                    if (v[k + w] > 0.f) ws[j + w] = max(ws[j + w], 1u << 24);
+                    border = min(border, ws[j + w] * 256u + 64u * 256u);
                 }
             }
+            // Where the root's last two places decide on a code (one element in 100000), the exact one does.
+            if (border < 128u * 256u)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    uint32_t rm, rs;
+                    random_bits(hash + (uint32_t)(o + j) * 0x9E3779B1u, rm, rs);
+                    ws[j] = __float_as_uint(__fsqrt_rn(v[8 * b + 4 * u + j]) * is) * 16u + rs;
+                }
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (v[8 * b + 4 * u + j] > 0.f) ws[j] = max(ws[j], 1u << 24);   // what is above zero keeps a code above zero
             store4((P*)e.p + i0 + o, p);
             *(uint32_t*)((uint8_t*)e.m + i0 + o) = top_bytes(wm);
             *(uint32_t*)((uint8_t*)e.v + i0 + o) = top_bytes(ws);

@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import operator
 
 import torch
 
@@ -81,7 +82,11 @@ class _on:
         self.back = torch.cuda.current_device()
         if self.back != self.device:
             torch.cuda.set_device(self.device)
-        return context(self.device)
+        ctx = _ctxs.get(self.device)
+        if ctx is None:
+            return context(self.device)
+        lib().tb_set_stream(ctx, torch._C._cuda_getCurrentRawStream(self.device))
+        return ctx
 
     def __exit__(self, *exc):
         if self.back != self.device:
@@ -89,11 +94,16 @@ class _on:
 
 
 def _same(*ts):
-    """The one device that the tensors are on."""
-    devices = {t.get_device() for t in ts if t is not None}
-    if len(devices) > 1:
-        raise TeenyError(1, "tensors must be on one device")
-    return devices.pop()
+    """Checks that the tensors are contiguous and on one CUDA device, and returns that."""
+    dev = ts[0].get_device()
+    for t in ts:
+        if t is None:
+            continue
+        if t.get_device() != dev or dev < 0:
+            raise TeenyError(1, "tensors must be on one CUDA device (no CPU fallback)")
+        if not t.is_contiguous():
+            raise TeenyError(2, "tensors must be contiguous")
+    return dev
 
 
 def _columns(N, dtype, *ts):
@@ -120,14 +130,15 @@ def layer_norm(x, w, b, eps=1e-5, return_stats=False):
     """layer_norm_forward_inference (nn/norm/layernorm.rs:43-157); with
     return_stats=True layer_norm_forward (:163): (y, mean, rstd), the row
     statistics f32 [M] that layer_norm_backward takes."""
-    _cuda(x, w, b)
+    if not return_stats:
+        _cuda(x, w, b)
     N = x.shape[-1]
     y = torch.empty_like(x)
     if return_stats:
         dev = _same(x, w, b)
         _columns(N, x.dtype, w, b)
         M = x.numel() // N
-        mean, rstd = torch.empty(2, M, device=x.device, dtype=torch.float32)
+        mean, rstd = x.new_empty(M, dtype=torch.float32), x.new_empty(M, dtype=torch.float32)
         with _on(dev) as ctx:
             check(ctx, lib().tb_layernorm_fwd_train(ctx, _dt(x), x.data_ptr(), w.data_ptr(), b.data_ptr(), y.data_ptr(),
                                                     mean.data_ptr(), rstd.data_ptr(), M, N, eps))
@@ -503,6 +514,14 @@ def _workspace(op, dtype, shape, device):
     return torch.empty(max(n.value, 16), dtype=torch.uint8, device=device), n.value
 
 
+def _bytes_for(op, like, *shape):
+    """A workspace as _workspace's, on the device of a tensor."""
+    n = ctypes.c_size_t(0)
+    check(None, lib().tb_workspace_bytes(TB_OP[op], TB_F32, (ctypes.c_int64 * len(shape))(*shape), len(shape),
+                                         ctypes.byref(n)))
+    return like.new_empty(max(n.value, 16), dtype=torch.uint8), n.value
+
+
 TB_OP.update({"rmsnorm_bwd": 9, "linear_bwd": 10, "attn_bwd": 11, "conv2d_bwd": 12, "layernorm_bwd": 13,
               "grad_norm": 14})
 
@@ -527,7 +546,6 @@ def layer_norm_backward(dy, x, w, mean, rstd, dw=None, db=None):
     """Backward of layer_norm_forward (nn/norm/layernorm.rs:163): returns (dx, dw, db)
     from the forward's mean and rstd (f32 [M]); dw and db (f32 [N]) accumulate into
     the given tensors (both or neither)."""
-    _cuda(dy, x, w, mean, rstd, dw, db)
     dev = _same(dy, x, w, mean, rstd, dw, db)
     N = x.shape[-1]
     M = x.numel() // N
@@ -541,9 +559,9 @@ def layer_norm_backward(dy, x, w, mean, rstd, dw=None, db=None):
     if accumulate:
         _columns(N, torch.float32, dw, db)
     else:
-        dw, db = torch.empty(2, N, device=x.device, dtype=torch.float32)
+        dw, db = x.new_empty(N, dtype=torch.float32), x.new_empty(N, dtype=torch.float32)
     dx = torch.empty_like(x)
-    ws, nb = _workspace("layernorm_bwd", _dt(x), (M, N), x.device)
+    ws, nb = _bytes_for("layernorm_bwd", x, M, N)
     with _on(dev) as ctx:
         check(ctx, lib().tb_layernorm_bwd(ctx, _dt(x), dy.data_ptr(), x.data_ptr(), w.data_ptr(), mean.data_ptr(),
                                           rstd.data_ptr(), dx.data_ptr(), dw.data_ptr(), db.data_ptr(), accumulate, M, N,
@@ -598,19 +616,26 @@ def conv2d_backward(dy, x, w, stride=1, pad=0):
 
 
 # -------------------------------------------------------------- optimiser ---
+_T = torch.Tensor
+_dtype_of = operator.attrgetter("dtype")
+
+
 def _listed(what, ts, numel=None):
-    """Checks a list of tensors of one type and device; returns that type, the sizes and the addresses."""
-    for t in ts:
-        if not t.is_cuda:
-            raise TeenyError(1, "tensors must be on a CUDA device (no CPU fallback)")
-        if not t.is_contiguous():
-            raise TeenyError(2, "tensors must be contiguous")
-    if len({t.dtype for t in ts}) > 1:
+    """Checks a list of contiguous CUDA tensors of one type and device; returns type, device, sizes and addresses."""
+    devices, dtypes = set(map(_T.get_device, ts)), set(map(_dtype_of, ts))
+    if -1 in devices:
+        raise TeenyError(1, "tensors must be on a CUDA device (no CPU fallback)")
+    if len(devices) > 1:
+        raise TeenyError(1, "tensors must be on one device")
+    if not all(map(_T.is_contiguous, ts)):
+        raise TeenyError(2, "tensors must be contiguous")
+    if len(dtypes) > 1:
         raise TeenyError(5, f"{what} must have one dtype")
-    sizes = [t.numel() for t in ts]
+    sizes = list(map(_T.numel, ts))
     if numel is not None and sizes != numel:
         raise TeenyError(2, f"{what} must match the parameters, tensor by tensor")
-    return ts[0].dtype if ts else None, sizes, [t.data_ptr() for t in ts]
+    return (dtypes.pop() if dtypes else None, devices.pop() if devices else torch.cuda.current_device(), sizes,
+            list(map(_T.data_ptr, ts)))
 
 
 def grad_norm(grads, max_norm=None):
@@ -618,19 +643,19 @@ def grad_norm(grads, max_norm=None):
     (norm, scale), scale = min(1, max_norm / (norm + 1e-6)) being what AdamW.step takes as
     grad_scale to clip the gradients to max_norm."""
     grads = list(grads)
-    dtype, sizes, ptrs = _listed("gradients", grads)
-    dev = _same(*grads) if grads else torch.cuda.current_device()
+    dtype, dev, sizes, ptrs = _listed("gradients", grads)
     if grads and dtype not in _DT:
         raise TeenyError(5, f"unsupported dtype {dtype}")
     n = len(grads)
-    out = torch.empty(2, device=torch.device("cuda", dev), dtype=torch.float32)
-    ws, nb = _workspace("grad_norm", TB_F32, (n,), out.device)
-    at = out.data_ptr()
+    norm = torch.empty(1, device=torch.device("cuda", dev), dtype=torch.float32)
+    scale = None if max_norm is None else torch.empty_like(norm)
+    ws, nb = _bytes_for("grad_norm", norm, n)
     with _on(dev) as ctx:
         check(ctx, lib().tb_grad_norm(ctx, _DT.get(dtype, TB_F32), (ctypes.c_uint64 * n)(*ptrs),
-                                      (ctypes.c_int64 * n)(*sizes), n, at, None if max_norm is None else at + 4,
-                                      0.0 if max_norm is None else max_norm, ws.data_ptr(), nb))
-    return out[:1] if max_norm is None else (out[:1], out[1:])
+                                      (ctypes.c_int64 * n)(*sizes), n, norm.data_ptr(),
+                                      None if scale is None else scale.data_ptr(), 0.0 if scale is None else max_norm,
+                                      ws.data_ptr(), nb))
+    return norm if scale is None else (norm, scale)
 
 
 class _AdamWHyper(ctypes.Structure):
@@ -649,7 +674,7 @@ class AdamW:
 
     params and grads: lists of contiguous CUDA tensors, f32 / f32, f32 / bf16 or bf16 / bf16;
     copies: bf16 tensors that get each step's f32 parameters.  The addresses are kept: step() refuses
-    to run once a tensor has been given other memory.  Tensors must not overlap.
+    to run once one of these has been given other memory.  Tensors must not overlap.
 
     state_bits=32: m and v are f32.  state_bits=8: m and s = sqrt(v) are float8_e4m3fn with a uint8
     exponent for each 256 elements (m_exp, s_exp): code * 2^(exp - 127), rounded up or down at random
@@ -670,8 +695,9 @@ class AdamW:
             raise TeenyError(5, "moments in 32 or 8 bits")
         if step_count < 0:
             raise TeenyError(1, "step_count must not be negative")
-        pd, sizes, pp = _listed("parameters", self.params)
-        gd, _, gp = _listed("gradients", self.grads, sizes)
+        pd, self.device, sizes, pp = _listed("parameters", self.params)
+        gd, gdev, _, gp = _listed("gradients", self.grads, sizes)
+        devices = {self.device, gdev}
         n = len(sizes)
         blocks = [-(-k // 256) for k in sizes]
         names = (("m", torch.float32, sizes), ("v", torch.float32, sizes)) if state_bits == 32 else (
@@ -685,25 +711,29 @@ class AdamW:
                 ts = [t.view(dtype) for t in ts]
             else:
                 ts = list(state[name])
-            d, _, at = _listed(name, ts, want)
+            d, dev, _, at = _listed(name, ts, want)
+            devices.add(dev)
             if n and d != dtype:
                 raise TeenyError(5, f"{name} must be {dtype}, got {d}")
             setattr(self, name, ts)
             ptrs.append(at)
         cp = [0] * n
         if self.copies is not None:
-            cd, _, cp = _listed("copies", self.copies, sizes)
+            cd, dev, _, cp = _listed("copies", self.copies, sizes)
+            devices.add(dev)
             if n and cd != torch.bfloat16:
                 raise TeenyError(5, f"copies must be bfloat16, got {cd}")
         if n and (pd not in _DT or gd not in _DT):
             raise TeenyError(5, f"unsupported dtypes {pd}, {gd}")
         lists = [self.params, self.grads, self.copies or []] + [getattr(self, name) for name, _, _ in names]
-        self.device = _same(*(t for ts in lists for t in ts)) if n else torch.cuda.current_device()
+        if n and len(devices) > 1:
+            raise TeenyError(1, "tensors must be on one device")
         exps = ptrs[2:] or [[0] * n, [0] * n]
         rows = (ctypes.c_uint64 * (8 * n))(*(f for row in zip(pp, gp, ptrs[0], ptrs[1], *exps, cp, sizes) for f in row))
         # the memory lives as long as the optimiser, whatever becomes of the tensors
         self._alive = [t.detach() for ts in lists for t in ts]
-        self._watched, self._at = [t for ts in lists for t in ts], [t.data_ptr() for t in self._alive]
+        self._watched = [t for ts in lists[:3] for t in ts]
+        self._at = list(map(_T.data_ptr, self._watched))
         self._hyper = _AdamWHyper(0.0, betas[0], betas[1], eps, weight_decay, 0, seed & 0xFFFFFFFF, None, None, None)
         self._step_dev, self._step = None, step_count
         if capturable:
@@ -736,7 +766,7 @@ class AdamW:
         self.lr).  grad_scale: such a tensor, which multiplies the gradients."""
         lr = self.lr if lr is None else lr
         h = self._hyper
-        if [t.data_ptr() for t in self._watched] != self._at:
+        if list(map(_T.data_ptr, self._watched)) != self._at:
             raise TeenyError(1, "a tensor has been given other memory: make a new AdamW with this one's state")
         if isinstance(lr, torch.Tensor):
             h.lr, h.lr_dev = 0.0, self._scalar("lr", lr)

@@ -95,26 +95,12 @@ def encode(x, u, root):
     return code.astype(np.uint8).reshape(-1)[:n], e.astype(np.uint8)
 
 
-def at_border(x, u):
-    """Where 2 units in x's last place decide which of two codes it gets (x >= 0)."""
-    n = len(x)
-    x, u = blocks(np.asarray(x, F)), blocks(np.asarray(u, np.uint32))
-    e = np.maximum(np.where(np.isfinite(x), x, F(0)).max(1).view(np.uint32).astype(np.int64) >> 23, 7) - 7
-    with np.errstate(over="ignore", invalid="ignore"):
-        y = x * power(254 - e)[:, None]
-    rest = (np.where(y < F(2.0 ** -6), y + F(2.0 ** -6), y).astype(F).view(np.uint32) + ((u << np.uint32(4)) | np.uint32(8)))
-    rest = (rest & np.uint32(0xFFFFF)).astype(np.int64)
-    return (np.minimum(rest, (1 << 20) - rest) <= 3).reshape(-1)[:n]
-
-
 def adamw8_moments(g, cm, em, cs, es, seed, t, tensor, b1, b2, scale):
-    """New (m codes, m exponents, s codes, s exponents, where an s code may be the next one) of one tensor; every operation
-    rounded to f32, but that the kernel's square root may be off by 2 units in the last place (2^-23 relative)."""
+    """New (m codes, m exponents, s codes, s exponents) of one tensor; every operation rounded to f32."""
     with np.errstate(over="ignore", invalid="ignore", under="ignore"):
         g = np.asarray(g, F) * F(scale)
         m = held(cm, em) * F(b1) + g * F(1 - b1)
         s = held(cs, es)
         s = np.sqrt(s * s * F(b2) + g * g * F(1 - b2))
         bits = random_bits(seed, t, tensor, len(g))
-        high = bits >> np.uint32(16)
-        return (*encode(m, bits & np.uint32(0xFFFF), False), *encode(s, high, True), at_border(s, high))
+        return (*encode(m, bits & np.uint32(0xFFFF), False), *encode(s, bits >> np.uint32(16), True))

@@ -85,7 +85,7 @@ def test_root_follows_a_falling_gradient():
     v = np.zeros(n)
     for t in range(1, 2 * T + 1):
         g = r.standard_normal(n) * (1.0 if t <= T else 0.01)
-        cm, em, cs, es, _ = u.adamw8_moments(g, cm, em, cs, es, 1, t, 0, 0.9, 0.999, 1.0)
+        cm, em, cs, es = u.adamw8_moments(g, cm, em, cs, es, 1, t, 0, 0.9, 0.999, 1.0)
         v = 0.999 * v + 0.001 * g * g
     s = u.held(cs, es).astype(np.float64)
     # a root's own deviation around the 32-bit one is some twenty percent; the mean over 512 has 1 %
