@@ -12,6 +12,7 @@ torch is used only for device memory and streams.
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import math
 import operator
@@ -650,11 +651,11 @@ def grad_norm(grads, max_norm=None):
     norm = torch.empty(1, device=torch.device("cuda", dev), dtype=torch.float32)
     scale = None if max_norm is None else torch.empty_like(norm)
     ws, nb = _bytes_for("grad_norm", norm, n)
+    ptrs, sizes = array.array("Q", ptrs), array.array("q", sizes)
     with _on(dev) as ctx:
-        check(ctx, lib().tb_grad_norm(ctx, _DT.get(dtype, TB_F32), (ctypes.c_uint64 * n)(*ptrs),
-                                      (ctypes.c_int64 * n)(*sizes), n, norm.data_ptr(),
-                                      None if scale is None else scale.data_ptr(), 0.0 if scale is None else max_norm,
-                                      ws.data_ptr(), nb))
+        check(ctx, lib().tb_grad_norm(ctx, _DT.get(dtype, TB_F32), ptrs.buffer_info()[0], sizes.buffer_info()[0], n,
+                                      norm.data_ptr(), None if scale is None else scale.data_ptr(),
+                                      0.0 if scale is None else max_norm, ws.data_ptr(), nb))
     return norm if scale is None else (norm, scale)
 
 
@@ -729,7 +730,7 @@ class AdamW:
         if n and len(devices) > 1:
             raise TeenyError(1, "tensors must be on one device")
         exps = ptrs[2:] or [[0] * n, [0] * n]
-        rows = (ctypes.c_uint64 * (8 * n))(*(f for row in zip(pp, gp, ptrs[0], ptrs[1], *exps, cp, sizes) for f in row))
+        rows = array.array("Q", [f for row in zip(pp, gp, ptrs[0], ptrs[1], *exps, cp, sizes) for f in row])
         # the memory lives as long as the optimiser, whatever becomes of the tensors
         self._alive = [t.detach() for ts in lists for t in ts]
         self._watched = [t for ts in lists[:3] for t in ts]
@@ -743,7 +744,7 @@ class AdamW:
             raise TeenyError(1, "betas in [0, 1), eps and weight_decay >= 0")
         self._handle = ctypes.c_void_p()
         with _on(self.device) as ctx:
-            check(ctx, lib().tb_adamw_create(ctx, _DT.get(pd, TB_F32), _DT.get(gd, TB_F32), state_bits, rows, n,
+            check(ctx, lib().tb_adamw_create(ctx, _DT.get(pd, TB_F32), _DT.get(gd, TB_F32), state_bits, rows.buffer_info()[0], n,
                                              ctypes.byref(self._handle)))
 
     def __del__(self):
