@@ -275,43 +275,62 @@ __global__ void __launch_bounds__(fwd_cta<NT>()) ln_fwd_kernel(const T* __restri
     }
 }
 
-// Any row: one CTA, three passes (the second and third find the row in L2).
-template <typename T, int V>
-__global__ void __launch_bounds__(1024) ln_fwd_wide_kernel(const T* __restrict__ x, const T* __restrict__ w,
-                                                           const T* __restrict__ b, T* __restrict__ y,
-                                                           float* __restrict__ mean, float* __restrict__ rstd, int64_t N,
-                                                           float eps) {
+// Any row: one CTA of 1024.  K > 0: K vectors a thread hold it; else three passes (the second
+// and third find the row in L2).
+constexpr int kWide = 1024;
+
+// f(vector, its first column) for a thread's vectors of a row.
+template <typename T, int V, int K, typename F>
+__device__ __forceinline__ void each_vector(int64_t N, F f) {
+    if (K) {
+#pragma unroll
+        for (int i = 0; i < K; i++) {
+            const int64_t c = (int64_t)(i * kWide + threadIdx.x) * V;
+            if (c < N) f(i, c);
+        }
+    } else {
+        for (int64_t c = (int64_t)threadIdx.x * V; c < N; c += kWide * V) f(0, c);
+    }
+}
+
+template <typename T, int V, int K>
+__global__ void __launch_bounds__(kWide) ln_fwd_wide_kernel(const T* __restrict__ x, const T* __restrict__ w,
+                                                            const T* __restrict__ b, T* __restrict__ y,
+                                                            float* __restrict__ mean, float* __restrict__ rstd, int64_t N,
+                                                            float eps) {
     __shared__ float2 red[2][32];
     const T* xr = x + (int64_t)blockIdx.x * N;
     T* yr = y + (int64_t)blockIdx.x * N;
     const float inv = 1.f / (float)N;
-    RowVec<T, V> v, g, h;
+    RowVec<T, V> v[K ? K : 1];
     float s = 0.f;
-    for (int64_t c = (int64_t)threadIdx.x * V; c < N; c += 1024 * V) {
-        v.load(xr + c);
+    if (K) each_vector<T, V, K>(N, [&](int i, int64_t c) { v[i].load(xr + c); });   // all in flight
+    each_vector<T, V, K>(N, [&](int i, int64_t c) {
+        if (!K) v[0].load(xr + c);
 #pragma unroll
-        for (int j = 0; j < V; j++) s += v.get(j);
-    }
-    const float mu = group_sum<1024, 1>(s, red[0]) * inv;
+        for (int j = 0; j < V; j++) s += v[i].get(j);
+    });
+    const float mu = group_sum<kWide, 1>(s, red[0]) * inv;
     float q = 0.f;
-    for (int64_t c = (int64_t)threadIdx.x * V; c < N; c += 1024 * V) {
-        v.load(xr + c);
+    each_vector<T, V, K>(N, [&](int i, int64_t c) {
+        if (!K) v[0].load(xr + c);
 #pragma unroll
         for (int j = 0; j < V; j++) {
-            const float d = v.get(j) - mu;
+            const float d = v[i].get(j) - mu;
             q += d * d;
         }
-    }
-    const float rs = rsqrtf(group_sum<1024, 1>(q, red[1]) * inv + eps);
-    for (int64_t c = (int64_t)threadIdx.x * V; c < N; c += 1024 * V) {
-        v.load(xr + c);
+    });
+    const float rs = rsqrtf(group_sum<kWide, 1>(q, red[1]) * inv + eps);
+    each_vector<T, V, K>(N, [&](int i, int64_t c) {
+        RowVec<T, V> g, h;
+        if (!K) v[0].load(xr + c);
         g.load(w + c);
         h.load(b + c);
         float o[V];
 #pragma unroll
-        for (int j = 0; j < V; j++) o[j] = (v.get(j) - mu) * rs * g.get(j) + h.get(j);
+        for (int j = 0; j < V; j++) o[j] = (v[i].get(j) - mu) * rs * g.get(j) + h.get(j);
         RowVec<T, V>::store(yr + c, o);
-    }
+    });
     if (threadIdx.x == 0) {
         mean[blockIdx.x] = mu;
         rstd[blockIdx.x] = rs;
@@ -432,40 +451,44 @@ __global__ void __launch_bounds__(bwd_cta<NT>()) ln_bwd_kernel(const T* __restri
     }
 }
 
-// Any row: dx by one CTA, two passes.
-template <typename T, int V>
-__global__ void __launch_bounds__(1024) ln_bwd_wide_dx_kernel(const T* __restrict__ dy, const T* __restrict__ x,
-                                                              const T* __restrict__ w, const float* __restrict__ mean,
-                                                              const float* __restrict__ rstd, T* __restrict__ dx,
-                                                              int64_t N) {
+// Any row: dx by one CTA, its vectors in registers (K > 0) or in two passes.
+template <typename T, int V, int K>
+__global__ void __launch_bounds__(kWide) ln_bwd_wide_dx_kernel(const T* __restrict__ dy, const T* __restrict__ x,
+                                                               const T* __restrict__ w, const float* __restrict__ mean,
+                                                               const float* __restrict__ rstd, T* __restrict__ dx,
+                                                               int64_t N) {
     __shared__ float2 red[32];
     const int64_t base = (int64_t)blockIdx.x * N;
     const float mu = mean[blockIdx.x], rs = rstd[blockIdx.x], inv = 1.f / (float)N;
-    RowVec<T, V> xv, gv, wv;
+    RowVec<T, V> xv[K ? K : 1], gv[K ? K : 1];
+    auto load = [&](int i, int64_t c) {
+        xv[i].load(x + base + c);
+        gv[i].load(dy + base + c);
+    };
+    if (K) each_vector<T, V, K>(N, load);   // all in flight
     float2 s = make_float2(0.f, 0.f);
-    for (int64_t c = (int64_t)threadIdx.x * V; c < N; c += 1024 * V) {
-        xv.load(x + base + c);
-        gv.load(dy + base + c);
+    each_vector<T, V, K>(N, [&](int i, int64_t c) {
+        RowVec<T, V> wv;
+        if (!K) load(0, c);
         wv.load(w + c);
 #pragma unroll
         for (int j = 0; j < V; j++) {
-            const float a = gv.get(j) * wv.get(j);
+            const float a = gv[i].get(j) * wv.get(j);
             s.x += a;
-            s.y += a * ((xv.get(j) - mu) * rs);
+            s.y += a * ((xv[i].get(j) - mu) * rs);
         }
-    }
-    s = group_sum2<1024, 1>(s.x, s.y, red);
+    });
+    s = group_sum2<kWide, 1>(s.x, s.y, red);
     const float c1 = s.x * inv, c2 = s.y * inv;
-    for (int64_t c = (int64_t)threadIdx.x * V; c < N; c += 1024 * V) {
-        xv.load(x + base + c);
-        gv.load(dy + base + c);
+    each_vector<T, V, K>(N, [&](int i, int64_t c) {
+        RowVec<T, V> wv;
+        if (!K) load(0, c);
         wv.load(w + c);
         float o[V];
 #pragma unroll
-        for (int j = 0; j < V; j++)
-            o[j] = rs * (gv.get(j) * wv.get(j) - c1 - (xv.get(j) - mu) * rs * c2);
+        for (int j = 0; j < V; j++) o[j] = rs * (gv[i].get(j) * wv.get(j) - c1 - (xv[i].get(j) - mu) * rs * c2);
         RowVec<T, V>::store(dx + base + c, o);
-    }
+    });
 }
 
 // Any rows: dw and db over the rows of split blockIdx.y, V columns a thread.
@@ -480,17 +503,28 @@ __global__ void __launch_bounds__(256) ln_bwd_wide_cols_kernel(const T* __restri
     float aw[V], ab[V];
 #pragma unroll
     for (int j = 0; j < V; j++) aw[j] = ab[j] = 0.f;
-    RowVec<T, V> xv, gv;
-#pragma unroll 4
-    for (int64_t r = r0; r < r1; r++) {
-        xv.load(x + r * N + c);
-        gv.load(dy + r * N + c);
-        const float mu = mean[r], rs = rstd[r];
+    for (int64_t r = r0; r < r1; r += 4) {   // four rows in flight
+        RowVec<T, V> xv[4], gv[4];
+        float mu[4], rs[4];
 #pragma unroll
-        for (int j = 0; j < V; j++) {
-            aw[j] += gv.get(j) * ((xv.get(j) - mu) * rs);
-            ab[j] += gv.get(j);
+        for (int k = 0; k < 4; k++) {
+            xv[k].zero();
+            gv[k].zero();
+            mu[k] = rs[k] = 0.f;
+            if (r + k < r1) {
+                xv[k].load(x + (r + k) * N + c);
+                gv[k].load(dy + (r + k) * N + c);
+                mu[k] = mean[r + k];
+                rs[k] = rstd[r + k];
+            }
         }
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                aw[j] += gv[k].get(j) * ((xv[k].get(j) - mu[k]) * rs[k]);
+                ab[j] += gv[k].get(j);
+            }
     }
     float* pw = part + (int64_t)blockIdx.y * 2 * N;
 #pragma unroll
@@ -558,11 +592,11 @@ int64_t bwd_ctas(int64_t M, int64_t N, int esz) {
     return ctas_for(M, N, esz, (nt % 3 ? 512 : 384) / nt, 1);
 }
 
-// Rows of partial sums that the several-pass backward writes: two CTAs an SM or so over tiles of 256 columns at
-// least, 16 rows a split at least.
+// Rows of partial sums that the several-pass backward writes: some six CTAs an SM over tiles of 2048 columns, 16
+// rows a split at least.
 int64_t wide_parts(int64_t M, int64_t N) {
     const int64_t tiles = (N + 2047) / 2048;
-    return std::max<int64_t>(1, std::min((2 * kLnSms + tiles - 1) / tiles, (M + 15) / 16));
+    return std::max<int64_t>(1, std::min((6 * kLnSms + tiles - 1) / tiles, (M + 15) / 16));
 }
 
 template <typename T>
@@ -570,8 +604,9 @@ int fwd(tb_ctx* ctx, const T* x, const T* w, const T* b, T* y, float* mean, floa
     constexpr int V = 16 / sizeof(T);
     if (!one_pass(N, sizeof(T)) || !aligned16(x) || !aligned16(y)) {
         const bool vec = N % V == 0 && aligned16(x) && aligned16(y) && aligned16(w) && aligned16(b);
-        return launch(ctx, "layernorm_fwd_wide", vec ? ln_fwd_wide_kernel<T, V> : ln_fwd_wide_kernel<T, 1>, dim3((unsigned)M),
-                      dim3(1024), 0, x, w, b, y, mean, rstd, N, eps);
+        constexpr int K = 16 / V;   // rows of up to 16384 in registers
+        auto kern = !vec ? ln_fwd_wide_kernel<T, 1, 0> : N <= kWide * 16 ? ln_fwd_wide_kernel<T, V, K> : ln_fwd_wide_kernel<T, V, 0>;
+        return launch(ctx, "layernorm_fwd_wide", kern, dim3((unsigned)M), dim3(kWide), 0, x, w, b, y, mean, rstd, N, eps);
     }
     const int nt = group_of(N, sizeof(T)), threads = nt == 32 ? 256 : nt;
     const int64_t grid = ctas_for(M, N, sizeof(T), threads / nt, fwd_ctas(threads));
@@ -608,8 +643,9 @@ int bwd(tb_ctx* ctx, const T* dy, const T* x, const T* w, const float* mean, con
         const bool vec = N % V == 0 && aligned16(x) && aligned16(dy) && aligned16(dx) && aligned16(w);
         const int cols = 256 * (vec ? V : 1);
         G = wide_parts(M, N);
-        rc = launch(ctx, "layernorm_bwd_wide", vec ? ln_bwd_wide_dx_kernel<T, V> : ln_bwd_wide_dx_kernel<T, 1>,
-                    dim3((unsigned)M), dim3(1024), 0, dy, x, w, mean, rstd, dx, N);
+        constexpr int K = 16 / V;   // rows of up to 16384 in registers
+        auto kern = !vec ? ln_bwd_wide_dx_kernel<T, 1, 0> : N <= kWide * 16 ? ln_bwd_wide_dx_kernel<T, V, K> : ln_bwd_wide_dx_kernel<T, V, 0>;
+        rc = launch(ctx, "layernorm_bwd_wide", kern, dim3((unsigned)M), dim3(kWide), 0, dy, x, w, mean, rstd, dx, N);
         if (rc) return rc;
         rc = launch(ctx, "layernorm_bwd_cols", vec ? ln_bwd_wide_cols_kernel<T, V> : ln_bwd_wide_cols_kernel<T, 1>,
                     dim3((unsigned)((N + cols - 1) / cols), (unsigned)G), dim3(256), 0, dy, x, mean, rstd, part, M, N,
