@@ -21,11 +21,24 @@
 // ends where the row does.  What a row's start is off a vector's is the same for
 // all rows of a group, since the grid's stride is a multiple of its period.
 //
-// Rows longer than a CTA's registers hold, and tensors that do not start at 16
-// bytes, take the kernels that read a row more than once.
+// Rows longer than a CTA's registers hold (8192 elements), and tensors that do not
+// start at 16 bytes, take the `wide` kernels: a CTA a row, which registers hold up
+// to 16384 elements, else passes over it; dw and db in a launch of their own.
+//
+// Measured on the device (inputs larger than L2; the floor is the bytes at the rate
+// of a copy, 6.45 TB/s): forward 16384 x 2048 bf16 22.1 us (floor 20.8), 4096 x 8192
+// f32 50 (41.6), 3001 x 5003 bf16 18 (9.3), 128 x 256 f32 2.1; backward 16384 x 2048
+// bf16 42.9 (31.2), of which 9 are the start and the sums of partial rows, 65536 x
+// 2048 145 (124.8), 2047 x 8192 f32 37.8 (31.2), 3001 x 5003 bf16 38 (14.0), 128 x
+// 256 f32 5.5.  What bounds the backward is the latency of a row's sums (shuffles,
+// barrier, shared memory) at the 16 warps that 128 registers a thread leave an SM:
+// two rows a barrier, or the next row's first half beside this one's second, cost
+// more instructions than they hid (47 us), and so did 24 warps that read a row twice
+// from the ring (54 us).
 #include <math.h>
 
 #include <algorithm>
+#include <initializer_list>
 #include <type_traits>
 
 #include "f32x2.cuh"
@@ -689,10 +702,23 @@ int bwd(tb_ctx* ctx, const T* dy, const T* x, const T* w, const float* mean, con
     return TB_OK;
 }
 
-// Whether the bytes at p meet those at q.
-bool meet(const void* p, size_t np, const void* q, size_t nq) {
-    const uintptr_t a = (uintptr_t)p, b = (uintptr_t)q;
-    return a < b + nq && b < a + np;
+struct Span {
+    const void* p;
+    size_t bytes;
+};
+// Whether one of the first `outs` spans meets another span.
+bool meet(const Span* s, int n, int outs) {
+    for (int i = 0; i < outs; i++)
+        for (int j = i + 1; j < n; j++) {
+            const uintptr_t a = (uintptr_t)s[i].p, b = (uintptr_t)s[j].p;
+            if (a < b + s[j].bytes && b < a + s[i].bytes) return true;
+        }
+    return false;
+}
+bool aligned_to(size_t a, std::initializer_list<const void*> ps) {
+    for (const void* p : ps)
+        if ((uintptr_t)p & (a - 1)) return false;
+    return true;
 }
 
 bool ln_shape_ok(int64_t M, int64_t N) {
@@ -716,8 +742,11 @@ int tb_layernorm_fwd_train(tb_ctx* ctx, int dtype, const void* x, const void* w,
     if (M == 0) return TB_OK;
     TB_REQUIRE(ctx, x && w && b && y && mean && rstd, TB_ERR_ARG, "layernorm_fwd_train: null pointer");
     const size_t es = dtype == TB_F32 ? 4 : 2, row = es * (size_t)N, all = row * (size_t)M;
-    TB_REQUIRE(ctx, !meet(y, all, x, all) && !meet(y, all, w, row) && !meet(y, all, b, row), TB_ERR_ARG,
-               "layernorm_fwd_train: y overlaps an input");
+    TB_REQUIRE(ctx, aligned_to(es, {x, w, b, y}) && aligned_to(4, {mean, rstd}), TB_ERR_ALIGN,
+               "layernorm_fwd_train: a pointer is not aligned to its type");
+    const size_t stat = 4 * (size_t)M;
+    const Span spans[] = {{y, all}, {mean, stat}, {rstd, stat}, {x, all}, {w, row}, {b, row}};
+    TB_REQUIRE(ctx, !meet(spans, 6, 3), TB_ERR_ARG, "layernorm_fwd_train: an output overlaps another tensor");
     if (dtype == TB_F32)
         return fwd(ctx, (const float*)x, (const float*)w, (const float*)b, (float*)y, mean, rstd, M, N, eps);
     return fwd(ctx, (const bf16*)x, (const bf16*)w, (const bf16*)b, (bf16*)y, mean, rstd, M, N, eps);
@@ -743,8 +772,12 @@ int tb_layernorm_bwd(tb_ctx* ctx, int dtype, const void* dy, const void* x, cons
                "layernorm_bwd: workspace of %zu bytes required (tb_workspace_bytes)", need);
     TB_REQUIRE(ctx, aligned16(workspace), TB_ERR_ALIGN, "layernorm_bwd: workspace must be 16-byte aligned");
     const size_t es = dtype == TB_F32 ? 4 : 2, row = es * (size_t)N, all = row * (size_t)M, sums = 4 * (size_t)N;
-    TB_REQUIRE(ctx, !meet(dx, all, x, all) && !meet(dx, all, dy, all) && !meet(dx, all, w, row) && !meet(dw, sums, db, sums),
-               TB_ERR_ARG, "layernorm_bwd: an output overlaps another tensor");
+    TB_REQUIRE(ctx, aligned_to(es, {dy, x, w, dx}) && aligned_to(4, {mean, rstd, dw, db}), TB_ERR_ALIGN,
+               "layernorm_bwd: a pointer is not aligned to its type");
+    const size_t stat = 4 * (size_t)M;
+    const Span spans[] = {{dx, all}, {dw, sums},   {db, sums},   {workspace, need}, {dy, all},
+                          {x, all},  {w, row},     {mean, stat}, {rstd, stat}};
+    TB_REQUIRE(ctx, !meet(spans, 9, 4), TB_ERR_ARG, "layernorm_bwd: an output overlaps another tensor");
     float* part = reinterpret_cast<float*>(workspace);
     if (dtype == TB_F32)
         return bwd(ctx, (const float*)dy, (const float*)x, (const float*)w, mean, rstd, (float*)dx, dw, db, accumulate, M, N,

@@ -133,10 +133,12 @@ def layer_norm(x, w, b, eps=1e-5, return_stats=False):
     statistics f32 [M] that layer_norm_backward takes."""
     if not return_stats:
         _cuda(x, w, b)
-    N = x.shape[-1]
+    N = x.shape[-1] if x.dim() else 0
     y = torch.empty_like(x)
     if return_stats:
         dev = _same(x, w, b)
+        if not N:
+            raise TeenyError(2, "rows of no elements")
         _columns(N, x.dtype, w, b)
         M = x.numel() // N
         mean, rstd = x.new_empty(M, dtype=torch.float32), x.new_empty(M, dtype=torch.float32)
@@ -548,7 +550,9 @@ def layer_norm_backward(dy, x, w, mean, rstd, dw=None, db=None):
     from the forward's mean and rstd (f32 [M]); dw and db (f32 [N]) accumulate into
     the given tensors (both or neither)."""
     dev = _same(dy, x, w, mean, rstd, dw, db)
-    N = x.shape[-1]
+    N = x.shape[-1] if x.dim() else 0
+    if not N:
+        raise TeenyError(2, "rows of no elements")
     M = x.numel() // N
     if dy.shape != x.shape or dy.dtype != x.dtype:
         raise TeenyError(2, f"dy is {tuple(dy.shape)} of {dy.dtype}, x {tuple(x.shape)} of {x.dtype}")
@@ -710,6 +714,8 @@ class AdamW:
                 ts = [torch.zeros(k, device=p.device, dtype=torch.uint8 if state_bits == 8 else dtype)
                       for k, p in zip(want, self.params)]
                 ts = [t.view(dtype) for t in ts]
+            elif name not in state:
+                raise TeenyError(1, f"state has no {name}")
             else:
                 ts = list(state[name])
             d, dev, _, at = _listed(name, ts, want)
@@ -737,6 +743,7 @@ class AdamW:
         self._at = list(map(_T.data_ptr, self._watched))
         self._hyper = _AdamWHyper(0.0, betas[0], betas[1], eps, weight_decay, 0, seed & 0xFFFFFFFF, None, None, None)
         self._step_dev, self._step = None, step_count
+        self._captured = []   # scalars that captured steps read at each replay
         if capturable:
             self._step_dev = torch.full((1,), step_count, device=torch.device("cuda", self.device), dtype=torch.int64)
             self._hyper.step_dev = self._step_dev.data_ptr()
@@ -746,6 +753,9 @@ class AdamW:
         with _on(self.device) as ctx:
             check(ctx, lib().tb_adamw_create(ctx, _DT.get(pd, TB_F32), _DT.get(gd, TB_F32), state_bits, rows.buffer_info()[0], n,
                                              ctypes.byref(self._handle)))
+
+    def __reduce__(self):
+        raise TypeError("an AdamW holds a handle of the library and cannot be copied: make another with its state")
 
     def __del__(self):
         if getattr(self, "_handle", None):
@@ -777,10 +787,12 @@ class AdamW:
             raise TeenyError(1, f"lr must not be negative, got {lr}")
         h.grad_scale = None if grad_scale is None else self._scalar("grad_scale", grad_scale)
         with _on(self.device) as ctx:
+            if torch.cuda.is_current_stream_capturing():
+                if self._step_dev is None:
+                    raise TeenyError(5, "a step whose count is on the host cannot be captured: AdamW(capturable=True)")
+                self._captured.append((lr, grad_scale))
             if self._step_dev is not None:
                 self._step_dev.add_(1)
-            elif torch.cuda.is_current_stream_capturing():
-                raise TeenyError(5, "a step whose count is on the host cannot be captured: AdamW(capturable=True)")
             h.step = self._step + 1
             check(ctx, lib().tb_adamw_step(self._handle, ctypes.byref(h)))
             self._step += 1

@@ -271,6 +271,9 @@ def test_refusals():
         lambda: o.layer_norm(x, w, w.bfloat16(), return_stats=True),
         lambda: o.layer_norm(x.half(), w.half(), w.half(), return_stats=True),
         lambda: o.layer_norm(x.t(), w, w, return_stats=True),
+        lambda: o.layer_norm(x[:, :0].contiguous(), w[:0], w[:0], return_stats=True),
+        lambda: o.layer_norm(x[0, 0], w[:1], w[:1], return_stats=True),
+        lambda: o.layer_norm_backward(x[:, :0].contiguous(), x[:, :0].contiguous(), w[:0], mean, rstd),
         lambda: o.layer_norm_backward(x[:2], x, w, mean, rstd),
         lambda: o.layer_norm_backward(x.bfloat16(), x, w, mean, rstd),
         lambda: o.layer_norm_backward(x, x, w, mean[:3], rstd),
@@ -299,3 +302,9 @@ def test_refusals():
     assert l.tb_layernorm_fwd_train(ctx, 0, x.data_ptr(), w.data_ptr(), w.data_ptr(), dx.data_ptr(), mean.data_ptr(),
                                     rstd.data_ptr(), 4, 0, 1e-5) == 2
     assert b"overlap" not in l.tb_last_error(ctx)
+    # between two floats; statistics in y; sums in the workspace
+    assert l.tb_layernorm_fwd_train(ctx, 0, x.data_ptr(), w.data_ptr() + 2, w.data_ptr(), dx.data_ptr(), mean.data_ptr(),
+                                    rstd.data_ptr(), 4, 8, 1e-5) == 3
+    assert l.tb_layernorm_fwd_train(ctx, 0, x.data_ptr(), w.data_ptr(), w.data_ptr(), dx.data_ptr(), dx.data_ptr(),
+                                    rstd.data_ptr(), 4, 8, 1e-5) == 1
+    assert l.tb_layernorm_bwd(*args, dx.data_ptr(), ws.data_ptr(), db.data_ptr(), 0, 4, 8, ws.data_ptr(), 1 << 20) == 1

@@ -1,4 +1,6 @@
 """The gradient norm and AdamW against 64 bits; the 8-bit moments bit for bit against their definition.  Tolerances: optim_util.bounds."""
+import copy
+
 import numpy as np
 import pytest
 
@@ -157,7 +159,7 @@ def test_adamw_from_nothing(bits):
 
 
 @pytest.mark.parametrize("hyper", [dict(b1=0.0, b2=0.0), dict(b1=0.0, b2=0.99, eps=1e-3, wd=0.0),
-                                   dict(b1=0.99, b2=0.95, lr=0.0, wd=0.5)])
+                                   dict(b1=0.99, b2=0.95, lr=0.0, wd=0.5), dict(eps=0.0), dict(eps=1e-31, b2=0.5)])
 @pytest.mark.parametrize("bits", [32, 8])
 def test_adamw_hyperparameters(bits, hyper):
     ops()
@@ -381,6 +383,44 @@ def test_adamw_refusals():
     with pytest.raises(E, match="other memory"):
         opt.step()
     assert opt.step_count == 0
+    with pytest.raises(E, match="has no v"):
+        o.AdamW([p], [g], state=dict(m=[t()]))
+    with pytest.raises(TypeError):
+        copy.copy(opt)
+
+
+def test_entry_points_refuse_bad_tables():
+    import ctypes
+
+    from teenygrad_b200 import lib
+    ctx = ops().context()
+    l, h = lib(), ctypes.c_void_p()
+    t = [torch.zeros(64, device="cuda") for _ in range(4)]
+    at = [x.data_ptr() for x in t]
+
+    def create(row, n=1, p=0, g=0, bits=32):
+        r = l.tb_adamw_create(ctx, p, g, bits, (ctypes.c_uint64 * len(row))(*row) if row else None, n, ctypes.byref(h))
+        if not r:
+            l.tb_adamw_destroy(h)
+        return r
+
+    good = at + [0, 0, 0, 64]
+    assert create(good) == 0
+    assert create(at[:3] + [0, 0, 0, 0, 64]) == 1            # no v
+    assert create([at[0] + 2] + good[1:]) == 3               # between floats
+    assert create(at + [0, 0, 0, (1 << 64) - 1]) == 2        # -1 elements
+    assert create(at + [0, 0, 0, 1 << 40]) == 2              # more than are counted
+    assert create(good, p=2) == 5 and create(good, p=1, g=0) == 5 and create(good, bits=16) == 5
+    assert create(good, bits=8) == 1                         # no exponents
+    assert create([], n=1) == 1 and create([], n=-1) == 1
+    assert create([at[0], at[1], at[0], at[3], 0, 0, 0, 64]) == 1   # m where p is
+    assert l.tb_grad_norm(ctx, 0, None, None, 1, at[0], None, 0.0, at[1], 256) == 1
+    assert l.tb_grad_norm(ctx, 0, None, None, 0, at[0], None, 0.0, None, 0) == 1
+    one, size = (ctypes.c_uint64 * 1)(at[0] + 1), (ctypes.c_int64 * 1)(8)
+    ws = torch.empty(1 << 16, device="cuda", dtype=torch.uint8)
+    assert l.tb_grad_norm(ctx, 0, one, size, 1, at[1], None, 0.0, ws.data_ptr(), 1 << 16) == 3
+    size[0] = -1
+    assert l.tb_grad_norm(ctx, 0, one, size, 1, at[1], None, 0.0, ws.data_ptr(), 1 << 16) == 2
 
 
 def test_a_step_counted_on_the_host_is_not_captured():
