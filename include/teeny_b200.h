@@ -274,8 +274,8 @@ TB_API int tb_layernorm_fwd_train(tb_ctx* ctx, int dtype, const void* x, const v
  * dx[m,n] = rstd[m] (a - sum_n(a) / N - xhat sum_n(a xhat) / N),
  * dw[n] = sum_m dy xhat, db[n] = sum_m dy (f32 [N]; added to what they hold when
  * `accumulate` is not 0, written otherwise).  Outputs must not overlap inputs.
- * M = 0 leaves or zeroes dw and db.  Workspace: TB_OP_LAYERNORM_BWD {M, N}, 16-byte
- * aligned. */
+ * M = 0 leaves or zeroes dw and db.  Workspace: TB_OP_LAYERNORM_BWD {M, N} of the
+ * dtype, 16-byte aligned (0 bytes, and then NULL, for few rows). */
 TB_API int tb_layernorm_bwd(tb_ctx* ctx, int dtype, const void* dy, const void* x, const void* w, const float* mean,
                             const float* rstd, void* dx, float* dw, float* db, int accumulate, int64_t M, int64_t N,
                             void* workspace, size_t workspace_bytes);

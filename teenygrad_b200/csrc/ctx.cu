@@ -204,7 +204,7 @@ int tb_workspace_bytes(int op, int dtype, const int64_t* shape, int n_shape, siz
         case TB_OP_LAYERNORM_BWD:   // {M, N}
             if (!shape || n_shape != 2) return TB_ERR_ARG;
             if (shape[0] < 0 || shape[0] >= (1ll << 31) || shape[1] <= 0 || shape[1] >= (1ll << 31)) return TB_ERR_SHAPE;
-            *bytes = tb_layernorm_bwd_ws(shape[0], shape[1]);
+            *bytes = tb_layernorm_bwd_ws(dtype, shape[0], shape[1]);
             return TB_OK;
         case TB_OP_GRAD_NORM:       // {tensors}
             if (!shape || n_shape != 1) return TB_ERR_ARG;

@@ -351,12 +351,26 @@ __global__ void __launch_bounds__(kWide) ln_fwd_wide_kernel(const T* __restrict_
 }
 
 // --------------------------------------------------------------- backward --
-// part: [gridDim.x][2][N], the CTA's sums of dw and db.
+// Where a launch's sums of dw and db go: row k of part, [2][N] each, or, of one CTA alone, the results.
+struct Sums {
+    float *part, *dw, *db;
+    int64_t N;
+    int accumulate;
+    __device__ __forceinline__ void put(int64_t k, int64_t rows, int64_t c, float v) const {
+        if (rows > 1) {
+            part[k * 2 * N + c] = v;
+            return;
+        }
+        float* out = c < N ? dw + c : db + (c - N);
+        *out = accumulate ? *out + v : v;
+    }
+};
+
 template <typename T, int VPT, int NT, bool SHIFT>
 __global__ void __launch_bounds__(bwd_cta<NT>()) ln_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x,
                                                               const T* __restrict__ w, const float* __restrict__ mean,
                                                               const float* __restrict__ rstd, T* __restrict__ dx,
-                                                              float* __restrict__ part, int64_t M, int N) {
+                                                              const Sums out, int64_t M, int N) {
     using C = Cols<T, VPT, NT, SHIFT>;
     constexpr int P = C::P, K = P * VPT, S = kLnStages, CTA = bwd_cta<NT>(), R = CTA / NT;
     extern __shared__ uint4 ring[];   // [S][x, dy][VPT][CTA]
@@ -455,12 +469,11 @@ __global__ void __launch_bounds__(bwd_cta<NT>()) ln_bwd_kernel(const T* __restri
                 }
         }
     __syncthreads();
-    float* pw = part + (int64_t)blockIdx.x * 2 * N;
     for (int c = threadIdx.x; c < 2 * N; c += CTA) {
         float v = sw[c];
 #pragma unroll
         for (int g = 1; g < R; g++) v += sw[g * 2 * N + c];
-        pw[c] = v;
+        out.put(blockIdx.x, gridDim.x, c, v);
     }
 }
 
@@ -508,8 +521,8 @@ __global__ void __launch_bounds__(kWide) ln_bwd_wide_dx_kernel(const T* __restri
 template <typename T, int V>
 __global__ void __launch_bounds__(256) ln_bwd_wide_cols_kernel(const T* __restrict__ dy, const T* __restrict__ x,
                                                                const float* __restrict__ mean,
-                                                               const float* __restrict__ rstd, float* __restrict__ part,
-                                                               int64_t M, int64_t N, int64_t rows) {
+                                                               const float* __restrict__ rstd, const Sums out, int64_t M,
+                                                               int64_t N, int64_t rows) {
     const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V;
     if (c >= N) return;
     const int64_t r0 = (int64_t)blockIdx.y * rows, r1 = r0 + rows < M ? r0 + rows : M;
@@ -539,11 +552,10 @@ __global__ void __launch_bounds__(256) ln_bwd_wide_cols_kernel(const T* __restri
                 ab[j] += gv[k].get(j);
             }
     }
-    float* pw = part + (int64_t)blockIdx.y * 2 * N;
 #pragma unroll
     for (int j = 0; j < V; j++) {
-        pw[c + j] = aw[j];
-        pw[N + c + j] = ab[j];
+        out.put(blockIdx.y, gridDim.y, c + j, aw[j]);
+        out.put(blockIdx.y, gridDim.y, N + c + j, ab[j]);
     }
 }
 
@@ -600,14 +612,26 @@ int64_t ctas_for(int64_t M, int64_t N, int esz, int rows, int ctas) {
 // 768 threads an SM, 1024 where a CTA has 512: fewer leave HBM idle, more wait for shared memory and for one another
 // (16384 x 2048 bf16 with 512 / 768 / 1024 / 1536: 24.4 / 22.1 / 25.6 / 24.1 us; 4096 x 8192 f32: 62 / 62 / 50 / 60).
 int fwd_ctas(int threads) { return (threads == 512 ? 1024 : 768) / threads; }
-int64_t bwd_ctas(int64_t M, int64_t N, int esz) {
+// CTAs of the backward: an SM's each; one alone, which writes the results itself, for up to two rows a group: as fast
+// (8 rows of 2048 bf16 7.1 us, 9 in several CTAs 7.1), with a launch and a workspace less for the host.  More rows a
+// group take a microsecond each (8 of them, 128 x 256 f32: 12.6 us, in several CTAs 5.6).
+int bwd_rows(int64_t N, int esz) {
     const int nt = group_of(N, esz);
-    return ctas_for(M, N, esz, (nt % 3 ? 512 : 384) / nt, 1);
+    return (nt % 3 ? 512 : 384) / nt;
+}
+bool bwd_alone(int64_t M, int64_t N, int esz) {
+    const int rows = bwd_rows(N, esz), V = 16 / esz;
+    if (!one_pass(N, esz) || M > 2 * rows) return false;
+    return N % V == 0 || rows % V == 0 || M <= rows;   // the stride keeps the rows' offsets, or there is none
+}
+int64_t bwd_ctas(int64_t M, int64_t N, int esz) {
+    return bwd_alone(M, N, esz) ? 1 : ctas_for(M, N, esz, bwd_rows(N, esz), 1);
 }
 
 // Rows of partial sums that the several-pass backward writes: some six CTAs an SM over tiles of 2048 columns, 16
 // rows a split at least.
-int64_t wide_parts(int64_t M, int64_t N) {
+int64_t wide_parts(int64_t M, int64_t N, int esz) {
+    if (bwd_alone(M, N, esz)) return 1;   // the workspace is asked for without the addresses
     const int64_t tiles = (N + 2047) / 2048;
     return std::max<int64_t>(1, std::min((6 * kLnSms + tiles - 1) / tiles, (M + 15) / 16));
 }
@@ -650,18 +674,19 @@ template <typename T>
 int bwd(tb_ctx* ctx, const T* dy, const T* x, const T* w, const float* mean, const float* rstd, T* dx, float* dw, float* db,
         int accumulate, int64_t M, int64_t N, float* part) {
     constexpr int V = 16 / sizeof(T);
+    const Sums out = {part, dw, db, N, accumulate};
     int64_t G;
     int rc;
     if (!one_pass(N, sizeof(T)) || !aligned16(x) || !aligned16(dy) || !aligned16(dx)) {
         const bool vec = N % V == 0 && aligned16(x) && aligned16(dy) && aligned16(dx) && aligned16(w);
         const int cols = 256 * (vec ? V : 1);
-        G = wide_parts(M, N);
+        G = wide_parts(M, N, sizeof(T));
         constexpr int K = 16 / V;   // rows of up to 16384 in registers
         auto kern = !vec ? ln_bwd_wide_dx_kernel<T, 1, 0> : N <= kWide * 16 ? ln_bwd_wide_dx_kernel<T, V, K> : ln_bwd_wide_dx_kernel<T, V, 0>;
         rc = launch(ctx, "layernorm_bwd_wide", kern, dim3((unsigned)M), dim3(kWide), 0, dy, x, w, mean, rstd, dx, N);
         if (rc) return rc;
         rc = launch(ctx, "layernorm_bwd_cols", vec ? ln_bwd_wide_cols_kernel<T, V> : ln_bwd_wide_cols_kernel<T, 1>,
-                    dim3((unsigned)((N + cols - 1) / cols), (unsigned)G), dim3(256), 0, dy, x, mean, rstd, part, M, N,
+                    dim3((unsigned)((N + cols - 1) / cols), (unsigned)G), dim3(256), 0, dy, x, mean, rstd, out, M, N,
                     (M + G - 1) / G);
     } else {
         const int nt = group_of(N, sizeof(T)), threads = nt % 3 ? 512 : 384;
@@ -669,7 +694,7 @@ int bwd(tb_ctx* ctx, const T* dy, const T* x, const T* w, const float* mean, con
         const int smem = kLnStages * 2 * threads * 16 * (int)sizeof(T);   // the groups' sums take 8 N bytes each, 64 KB at most
         auto go = [&](auto kern) {
             TB_CUDA_TRY(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-            return launch(ctx, "layernorm_bwd", kern, dim3((unsigned)G), dim3(threads), smem, dy, x, w, mean, rstd, dx, part,
+            return launch(ctx, "layernorm_bwd", kern, dim3((unsigned)G), dim3(threads), smem, dy, x, w, mean, rstd, dx, out,
                           M, (int)N);
         };
         auto of = [&](auto shift) {
@@ -687,7 +712,7 @@ int bwd(tb_ctx* ctx, const T* dy, const T* x, const T* w, const float* mean, con
         };
         rc = N % V ? of(std::true_type()) : of(std::false_type());
     }
-    if (rc) return rc;
+    if (rc || G == 1) return rc;
     // launched while the last CTAs still run: it waits for them itself
     cudaLaunchConfig_t lc = {};
     lc.gridDim = dim3((unsigned)((2 * N + 31) / 32));
@@ -767,8 +792,8 @@ int tb_layernorm_bwd(tb_ctx* ctx, int dtype, const void* dy, const void* x, cons
         return TB_OK;
     }
     TB_REQUIRE(ctx, dy && x && w && mean && rstd && dx, TB_ERR_ARG, "layernorm_bwd: null pointer");
-    const size_t need = tb_layernorm_bwd_ws(M, N);
-    TB_REQUIRE(ctx, workspace && workspace_bytes >= need, TB_ERR_ARG,
+    const size_t need = tb_layernorm_bwd_ws(dtype, M, N);
+    TB_REQUIRE(ctx, !need || (workspace && workspace_bytes >= need), TB_ERR_ARG,
                "layernorm_bwd: workspace of %zu bytes required (tb_workspace_bytes)", need);
     TB_REQUIRE(ctx, aligned16(workspace), TB_ERR_ALIGN, "layernorm_bwd: workspace must be 16-byte aligned");
     const size_t es = dtype == TB_F32 ? 4 : 2, row = es * (size_t)N, all = row * (size_t)M, sums = 4 * (size_t)N;
@@ -785,13 +810,13 @@ int tb_layernorm_bwd(tb_ctx* ctx, int dtype, const void* dy, const void* x, cons
     return bwd(ctx, (const bf16*)dy, (const bf16*)x, (const bf16*)w, mean, rstd, (bf16*)dx, dw, db, accumulate, M, N, part);
 }
 
-size_t tb_layernorm_bwd_ws(int64_t M, int64_t N) {
+size_t tb_layernorm_bwd_ws(int dtype, int64_t M, int64_t N) {
     if (!ln_shape_ok(M, N) || !M) return 0;
-    // enough for either type and either kernel
-    int64_t parts = wide_parts(M, N);
-    for (int esz = 2; esz <= 4; esz += 2)
-        if (one_pass(N, esz)) parts = std::max(parts, bwd_ctas(M, N, esz));
-    return (size_t)parts * 2 * (size_t)N * 4;
+    const int esz = dtype == TB_F32 ? 4 : 2;
+    // enough for either kernel
+    int64_t parts = wide_parts(M, N, esz);
+    if (one_pass(N, esz)) parts = std::max(parts, bwd_ctas(M, N, esz));
+    return parts > 1 ? (size_t)parts * 2 * (size_t)N * 4 : 0;
 }
 
 }  // extern "C"

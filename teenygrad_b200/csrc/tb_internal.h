@@ -55,7 +55,7 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 // Workspace of the backward ops (backward.cu); tb_workspace_bytes forwards to it.
 extern "C" int tb_backward_workspace_bytes(int op, int dtype, const int64_t* shape, int n_shape, size_t* bytes);
 // Workspaces of the LayerNorm backward (layernorm.cu) and the gradient norm (optim.cu); 0 for a bad shape.
-extern "C" size_t tb_layernorm_bwd_ws(int64_t M, int64_t N);
+extern "C" size_t tb_layernorm_bwd_ws(int dtype, int64_t M, int64_t N);
 extern "C" size_t tb_grad_norm_ws(int64_t n);
 
 namespace tb {

@@ -518,11 +518,11 @@ def _workspace(op, dtype, shape, device):
 
 
 def _bytes_for(op, like, *shape):
-    """A workspace as _workspace's, on the device of a tensor."""
+    """A workspace as _workspace's, for the type and on the device of a tensor: None where none is needed."""
     n = ctypes.c_size_t(0)
-    check(None, lib().tb_workspace_bytes(TB_OP[op], TB_F32, (ctypes.c_int64 * len(shape))(*shape), len(shape),
+    check(None, lib().tb_workspace_bytes(TB_OP[op], _dt(like), (ctypes.c_int64 * len(shape))(*shape), len(shape),
                                          ctypes.byref(n)))
-    return like.new_empty(max(n.value, 16), dtype=torch.uint8), n.value
+    return like.new_empty(n.value, dtype=torch.uint8) if n.value else None, n.value
 
 
 TB_OP.update({"rmsnorm_bwd": 9, "linear_bwd": 10, "attn_bwd": 11, "conv2d_bwd": 12, "layernorm_bwd": 13,
@@ -570,7 +570,7 @@ def layer_norm_backward(dy, x, w, mean, rstd, dw=None, db=None):
     with _on(dev) as ctx:
         check(ctx, lib().tb_layernorm_bwd(ctx, _dt(x), dy.data_ptr(), x.data_ptr(), w.data_ptr(), mean.data_ptr(),
                                           rstd.data_ptr(), dx.data_ptr(), dw.data_ptr(), db.data_ptr(), accumulate, M, N,
-                                          ws.data_ptr(), nb))
+                                          None if ws is None else ws.data_ptr(), nb))
     return dx, dw, db
 
 

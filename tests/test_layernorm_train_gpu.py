@@ -134,7 +134,12 @@ def test_mean_far_from_zero_and_constant_rows():
 
 def test_gradient_sums_accumulate():
     o = ops()
-    x, w, _, dy = inputs(100, 520, torch.bfloat16, seed=3)
+    for M in (3, 100, 2000):   # one CTA, and more
+        sums_accumulate(o, M)
+
+
+def sums_accumulate(o, M):
+    x, w, _, dy = inputs(M, 520, torch.bfloat16, seed=3)
     r = rng(1)
     dw0, db0 = r.standard_normal(520).astype(np.float32), r.standard_normal(520).astype(np.float32)
     g = [to_gpu(a, torch.bfloat16) for a in (dy, x, w)]
@@ -264,8 +269,9 @@ def test_on_another_stream_and_replayed():
 def test_refusals():
     o = ops()
     from teenygrad_b200 import TeenyError
-    x, w = torch.ones(4, 8, device="cuda"), torch.ones(8, device="cuda")
-    mean, rstd = torch.ones(4, device="cuda"), torch.ones(4, device="cuda")
+    M = 200
+    x, w = torch.ones(M, 8, device="cuda"), torch.ones(8, device="cuda")
+    mean, rstd = torch.ones(M, device="cuda"), torch.ones(M, device="cuda")
     bad = [
         lambda: o.layer_norm(x, w[:4], w, return_stats=True),
         lambda: o.layer_norm(x, w, w.bfloat16(), return_stats=True),
@@ -292,19 +298,19 @@ def test_refusals():
     args = (ctx, 0, x.data_ptr(), x.data_ptr(), w.data_ptr(), mean.data_ptr(), rstd.data_ptr())
     ws = torch.empty(1 << 20, device="cuda", dtype=torch.uint8)
     dx, dw, db = torch.empty_like(x), torch.empty_like(w), torch.empty_like(w)
-    tail = (dw.data_ptr(), db.data_ptr(), 0, 4, 8)
+    tail = (dw.data_ptr(), db.data_ptr(), 0, M, 8)
     l = lib()
     assert l.tb_layernorm_bwd(*args, dx.data_ptr(), *tail, ws.data_ptr(), 16) == 1          # too small a workspace
     assert l.tb_layernorm_bwd(*args, dx.data_ptr(), *tail, ws.data_ptr() + 4, 1 << 19) == 3  # at an odd address
     assert l.tb_layernorm_bwd(*args, x.data_ptr(), *tail, ws.data_ptr(), 1 << 20) == 1       # in place
     assert l.tb_layernorm_fwd_train(ctx, 0, x.data_ptr(), w.data_ptr(), w.data_ptr(), x.data_ptr(), mean.data_ptr(),
-                                    rstd.data_ptr(), 4, 8, 1e-5) == 1
+                                    rstd.data_ptr(), M, 8, 1e-5) == 1
     assert l.tb_layernorm_fwd_train(ctx, 0, x.data_ptr(), w.data_ptr(), w.data_ptr(), dx.data_ptr(), mean.data_ptr(),
-                                    rstd.data_ptr(), 4, 0, 1e-5) == 2
+                                    rstd.data_ptr(), M, 0, 1e-5) == 2
     assert b"overlap" not in l.tb_last_error(ctx)
     # between two floats; statistics in y; sums in the workspace
     assert l.tb_layernorm_fwd_train(ctx, 0, x.data_ptr(), w.data_ptr() + 2, w.data_ptr(), dx.data_ptr(), mean.data_ptr(),
-                                    rstd.data_ptr(), 4, 8, 1e-5) == 3
+                                    rstd.data_ptr(), M, 8, 1e-5) == 3
     assert l.tb_layernorm_fwd_train(ctx, 0, x.data_ptr(), w.data_ptr(), w.data_ptr(), dx.data_ptr(), dx.data_ptr(),
-                                    rstd.data_ptr(), 4, 8, 1e-5) == 1
-    assert l.tb_layernorm_bwd(*args, dx.data_ptr(), ws.data_ptr(), db.data_ptr(), 0, 4, 8, ws.data_ptr(), 1 << 20) == 1
+                                    rstd.data_ptr(), M, 8, 1e-5) == 1
+    assert l.tb_layernorm_bwd(*args, dx.data_ptr(), ws.data_ptr(), db.data_ptr(), 0, M, 8, ws.data_ptr(), 1 << 20) == 1

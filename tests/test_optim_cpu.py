@@ -122,9 +122,10 @@ def test_workspaces_need_no_gpu():
     def ask(op, *shape):
         return l.tb_workspace_bytes(op, 0, (ctypes.c_int64 * len(shape))(*shape), len(shape), ctypes.byref(b))
 
-    assert ask(13, 16, 64) == 0 and b.value >= 2 * 64 * 4 and b.value % (2 * 64 * 4) == 0
-    assert ask(13, 0, 64) == 0
-    assert ask(13, 1, 100000) == 0 and b.value == 2 * 100000 * 4
+    assert ask(13, 1000, 64) == 0 and b.value >= 2 * 64 * 4 and b.value % (2 * 64 * 4) == 0
+    assert ask(13, 0, 64) == 0 and b.value == 0
+    assert ask(13, 1, 100000) == 0 and b.value == 0      # the sums of one CTA's rows are the results
+    assert ask(13, 17, 100000) == 0 and b.value == 2 * 2 * 100000 * 4
     assert ask(13, 16) == 1 and ask(13, -1, 8) == 2 and ask(13, 8, 0) == 2 and ask(13, 1 << 31, 8) == 2
     assert ask(14, 3) == 0 and b.value > 0
     one = b.value
