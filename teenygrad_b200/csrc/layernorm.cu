@@ -26,11 +26,11 @@
 // to 16384 elements, else passes over it; dw and db in a launch of their own.
 //
 // Measured on the device (inputs larger than L2; the floor is the bytes at the rate
-// of a copy, 6.45 TB/s): forward 16384 x 2048 bf16 22.1 us (floor 20.8), 4096 x 8192
-// f32 50 (41.6), 3001 x 5003 bf16 18 (9.3), 128 x 256 f32 2.1; backward 16384 x 2048
-// bf16 42.9 (31.2), of which 9 are the start and the sums of partial rows, 65536 x
-// 2048 145 (124.8), 2047 x 8192 f32 37.8 (31.2), 3001 x 5003 bf16 38 (14.0), 128 x
-// 256 f32 5.5.  What bounds the backward is the latency of a row's sums (shuffles,
+// of a copy, 6.45 TB/s): forward 16384 x 2048 bf16 21.6 us (floor 20.8), 4096 x 8192
+// f32 47 (41.6), 3001 x 5003 bf16 18 (9.3), 128 x 256 f32 2.1; backward 16384 x 2048
+// bf16 41.2 (31.2), of which 8 are the start and the sums of partial rows, 65536 x
+// 2048 145 (124.8), 2047 x 8192 f32 37.5 (31.2), 3001 x 5003 bf16 38 (14.0), 128 x
+// 256 f32 5.6.  What bounds the backward is the latency of a row's sums (shuffles,
 // barrier, shared memory) at the 16 warps that 128 registers a thread leave an SM:
 // two rows a barrier, or the next row's first half beside this one's second, cost
 // more instructions than they hid (47 us), and so did 24 warps that read a row twice
