@@ -16,6 +16,7 @@ import array
 import ctypes
 import math
 import operator
+import threading
 
 import torch
 
@@ -71,8 +72,13 @@ _i64 = ctypes.c_int64
 _f = ctypes.c_float
 
 
+_context_lock = threading.Lock()
+
+
 class _on:
-    """The context of a device, which is the current one inside the block."""
+    """The context of a device, which is the current one inside the block.  The context's stream is the
+    calling thread's until the block ends: another thread that enters one waits (operators that use context()
+    alone do not)."""
 
     __slots__ = ("device", "back")
 
@@ -81,15 +87,21 @@ class _on:
 
     def __enter__(self):
         self.back = torch.cuda.current_device()
-        if self.back != self.device:
-            torch.cuda.set_device(self.device)
-        ctx = _ctxs.get(self.device)
-        if ctx is None:
-            return context(self.device)
-        lib().tb_set_stream(ctx, torch._C._cuda_getCurrentRawStream(self.device))
-        return ctx
+        _context_lock.acquire()
+        try:
+            if self.back != self.device:
+                torch.cuda.set_device(self.device)
+            ctx = _ctxs.get(self.device)
+            if ctx is None:
+                return context(self.device)
+            lib().tb_set_stream(ctx, torch._C._cuda_getCurrentRawStream(self.device))
+            return ctx
+        except BaseException:
+            self.__exit__()
+            raise
 
     def __exit__(self, *exc):
+        _context_lock.release()
         if self.back != self.device:
             torch.cuda.set_device(self.back)
 

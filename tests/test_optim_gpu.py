@@ -1,5 +1,6 @@
 """The gradient norm and AdamW against 64 bits; the 8-bit moments bit for bit against their definition.  Tolerances: optim_util.bounds."""
 import copy
+import threading
 
 import numpy as np
 import pytest
@@ -327,6 +328,46 @@ def test_adamw_on_another_stream():
         ob.step()
     torch.cuda.synchronize()
     assert torch.equal(a.params[0], b.params[0])
+
+
+def test_two_threads_on_streams_of_their_own():
+    """Each thread's calls go to its own stream, whatever the other one does meanwhile."""
+    o = ops()
+    x = [torch.randn(300, 1000, device="cuda") for _ in range(2)]
+    w = torch.rand(1000, device="cuda")
+    models = [Model([30000, 77], F32, F32, False, bits, seed=7) for bits in (32, 8)]
+    alone = [Model([30000, 77], F32, F32, False, bits, seed=7) for bits in (32, 8)]
+    opts, refs = [m.optimiser() for m in models], [m.optimiser() for m in alone]
+    want = [o.layer_norm(t, w, w, return_stats=True) for t in x]
+    for r in refs:
+        for _ in range(100):
+            r.step()
+    norms = [o.grad_norm([t]) for t in x]
+    torch.cuda.synchronize()
+    streams, bad = [torch.cuda.Stream() for _ in x], []
+
+    def work(k):
+        try:
+            with torch.cuda.stream(streams[k]):
+                for _ in range(100):
+                    y = o.layer_norm(x[k], w, w, return_stats=True)
+                    got = o.grad_norm([x[k]])
+                    opts[k].step()
+                    # read on this stream: what another stream wrote would be late
+                    if not (all(torch.equal(a, b) for a, b in zip(y, want[k])) and torch.equal(got, norms[k])):
+                        bad.append(k)
+        except Exception as e:   # pragma: no cover - shown by the assertion
+            bad.append(e)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not bad
+    for m, a in zip(models, alone):
+        assert all(torch.equal(p, q) for p, q in zip(m.params, a.params))
 
 
 def test_adamw_refusals():
