@@ -611,3 +611,42 @@ def test_a_training_step(bits):
                                                  flat(moments[k][1]), t, 1e-2, 0.9, 0.999, 1e-8, 0.01, c)
             _, bp = u.bounds(flat(before[k]), up, size, div)
             assert np.all(np.abs(flat(host(p)) - ref) <= bp)
+
+
+# ------------------------------------------------------- small numbers, eps --
+def fresh(m):
+    """Makes a Model's 8-bit moments those before the first step."""
+    for name, held in (("m", m.m), ("s", m.s)):
+        for k, n in enumerate(m.sizes):
+            held[k] = (np.zeros(n, np.uint8), np.zeros(-(-n // 256), np.uint8))
+            m.codes[name][k].zero_()
+            m.codes[name + "_exp"][k].zero_()
+
+
+@pytest.mark.parametrize("eps", [1e-10, 1e-12, 1e-15, 1e-20, 1e-25])
+@pytest.mark.parametrize("pt,gt,copy", TYPES)
+def test_adamw_8_bits_where_the_root_is_next_to_a_small_eps(pt, gt, copy, eps):
+    """Second moments under 2^-126 in blocks of ordinary ones, whose roots are what an eps as small is added to."""
+    ops()
+    n = 512 * 5 + 100
+    m = Model([n], pt, gt, copy, 8, seed=41)
+    r = rng(3)
+    g = r.standard_normal(n) * 1e-3
+    tiny = r.random(n) < 0.3
+    g[tiny] = (10.0 ** r.uniform(-19, np.log10(3e-18), n) * r.choice([-1, 1], n))[tiny]
+    g[1024:1536] = 1e-3    # a unit of whole blocks that has none
+    m.g[0] = rounded(g, gt)
+    m.grads[0].copy_(torch.from_numpy(m.g[0]))
+    for t in (1, 1000):
+        fresh(m)
+        m.optimiser(step_count=t - 1, eps=eps).step()
+        zero = np.zeros(n)
+        p, _, v, up, size, div = u.adamw64(m.p[0], m.g[0], zero, zero, t, LR, B1, B2, eps, WD, 1.0)
+        _, bound = u.bounds(m.p[0], up, size, div, p if pt == BF16 else None)
+        # under 2^-126 f32 has steps of 2^-149: half of one each for the square and its product, halved by the root
+        bound = bound + np.abs(up) * 2.0 ** -149 / (2 * np.maximum(v, 2.0 ** -149))
+        got = host(m.params[0])
+        assert np.all(np.abs(got - p) <= bound), np.max(np.abs(got - p) / bound)
+        m.check_codes(0, u.adamw8_moments(m.g[0], zero.astype(np.uint8), np.zeros(-(-n // 256), np.uint8), zero.astype(np.uint8),
+                                          np.zeros(-(-n // 256), np.uint8), 0, t, 0, B1, B2, 1.0))
+        m.p[0] = got
