@@ -3,7 +3,9 @@
  * operator surface.
  *
  * Every entry point takes device pointers and plain sizes, enqueues work on the
- * context's stream (no implicit synchronisation) and returns a tb_status.  The
+ * context's stream (no implicit synchronisation) and returns a tb_status.  A
+ * context (and what is created from it) serves one host thread at a time, from
+ * tb_set_stream to the return of the calls on that stream and tb_last_error.  The
  * reference executes one RuntimeOp per graph node: it packs kernel arguments
  * (RuntimeOp::pack_args, core/teeny-core/src/model/mod.rs:145), computes a grid
  * (RuntimeOp::grid, model/mod.rs:156) and launches teenyc-compiled PTX through

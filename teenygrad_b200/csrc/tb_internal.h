@@ -18,7 +18,7 @@ struct tb_ctx {
     int* d_err = nullptr;           // device error word (bounded-wait timeouts)
     std::string last_error;
     void* comm = nullptr;           // NCCL communicator state (comm.cu)
-    bool pdl = false;               // launch with programmatic stream serialization
+    bool pdl = false;               // launch with programmatic stream serialization; set within one call alone
     unsigned* chain_sync = nullptr; // tb_linear_chain_fwd scratch (allocated on first use)
     uint64_t* chain_ll = nullptr;
     size_t chain_ll_words = 0;
@@ -61,7 +61,8 @@ extern "C" size_t tb_grad_norm_ws(int64_t n);
 namespace tb {
 
 // cudaLaunchKernelEx on ctx->stream; adds the programmatic-serialization
-// attribute when ctx->pdl is set (the kernel must call pdl_wait()).
+// attribute when ctx->pdl is set: the kernels of the calls that set it call
+// pdl_wait().  Others never meet it, as a context serves one thread at a time.
 template <typename... KArgs, typename... Args>
 int launch(tb_ctx* ctx, const char* what, void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem,
            Args&&... args) {

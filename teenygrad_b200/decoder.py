@@ -16,7 +16,7 @@ from dataclasses import dataclass
 import torch
 
 from ._lib import TB_BF16, TB_F32, TeenyError, check, lib
-from .ops import context
+from .ops import _on
 
 P_EMBED, P_ATTN_NORM, P_WQ, P_WK, P_WV, P_WO, P_MLP_NORM = 0, 1, 2, 3, 4, 5, 6
 P_W_GATE, P_W_UP, P_W_DOWN, P_FINAL_NORM, P_LM_HEAD = 7, 8, 9, 10, 11
@@ -60,10 +60,11 @@ class Decoder:
     def __init__(self, cfg: DecoderConfig, device: int | None = None):
         self.cfg = cfg
         self.device = torch.cuda.current_device() if device is None else device
-        self.ctx = context(self.device)
         self._h = ctypes.c_void_p()
         c = cfg._c()
-        check(self.ctx, lib().tb_decoder_create(self.ctx, ctypes.byref(c), ctypes.byref(self._h)))
+        with _on(self.device) as ctx:
+            self.ctx = ctx
+            check(ctx, lib().tb_decoder_create(ctx, ctypes.byref(c), ctypes.byref(self._h)))
         self.B = 0
 
     def close(self):
@@ -76,9 +77,6 @@ class Decoder:
             self.close()
         except Exception:
             pass
-
-    def _ctx(self):
-        return context(self.device)
 
     # ---------------------------------------------------------- params --
     def set_param(self, kind: int, tensor, layer: int = 0):
@@ -95,9 +93,9 @@ class Decoder:
             ptr = keep.data_ptr()
             dt = TB_F32 if keep.dtype == torch.float32 else TB_BF16
             host = 0 if keep.is_cuda else 1
-        self._ctx()
-        check(self.ctx, lib().tb_decoder_set_param(self._h, ctypes.c_int(layer), ctypes.c_int(kind),
-                                                   ctypes.c_void_p(ptr), ctypes.c_int(dt), ctypes.c_int(host)))
+        with _on(self.device) as ctx:
+            check(ctx, lib().tb_decoder_set_param(self._h, ctypes.c_int(layer), ctypes.c_int(kind),
+                                                  ctypes.c_void_p(ptr), ctypes.c_int(dt), ctypes.c_int(host)))
 
     def set_param_int8(self, kind: int, q, scale, layer: int = 0):
         """int8 weight [rows, cols] + f32 scale [rows] (teeny-quant's I8 + _scale), numpy or torch."""
@@ -108,26 +106,26 @@ class Decoder:
         else:
             qk, sk = q.contiguous(), scale.float().contiguous()
             qp, sp, host = qk.data_ptr(), sk.data_ptr(), 0 if qk.is_cuda else 1
-        self._ctx()
-        check(self.ctx, lib().tb_decoder_set_param_int8(self._h, ctypes.c_int(layer), ctypes.c_int(kind),
-                                                        ctypes.c_void_p(qp), ctypes.c_void_p(sp), ctypes.c_int(host)))
+        with _on(self.device) as ctx:
+            check(ctx, lib().tb_decoder_set_param_int8(self._h, ctypes.c_int(layer), ctypes.c_int(kind),
+                                                       ctypes.c_void_p(qp), ctypes.c_void_p(sp), ctypes.c_int(host)))
 
     def load_checkpoint(self, path: str):
         """Loads a Llama-layout .safetensors checkpoint (F32 / BF16, or teeny-quant
         int8 with per-channel scales) and prepares the decoder."""
         from .checkpoint import SafeTensors
         with SafeTensors(path) as st:
-            self._ctx()
-            check(self.ctx, lib().tb_decoder_load_safetensors(self._h, st._h))
+            with _on(self.device) as ctx:
+                check(ctx, lib().tb_decoder_load_safetensors(self._h, st._h))
 
     def init_random(self, seed: int = 0, std: float = 0.02):
-        self._ctx()
-        check(self.ctx, lib().tb_decoder_init_random(self._h, ctypes.c_uint64(seed), ctypes.c_float(std)))
+        with _on(self.device) as ctx:
+            check(ctx, lib().tb_decoder_init_random(self._h, ctypes.c_uint64(seed), ctypes.c_float(std)))
         self.prepare()
 
     def prepare(self):
-        self._ctx()
-        check(self.ctx, lib().tb_decoder_prepare(self._h))
+        with _on(self.device) as ctx:
+            check(ctx, lib().tb_decoder_prepare(self._h))
 
     # --------------------------------------------------------- running --
     def prefill(self, ids: torch.Tensor, return_logits: bool = False):
@@ -135,25 +133,25 @@ class Decoder:
         assert ids.is_cuda and ids.dtype == torch.int32
         ids = ids.contiguous()
         B, S = ids.shape
-        self._ctx()
         nxt = torch.empty(B, device=ids.device, dtype=torch.int32)
         logits = torch.empty(B, self.cfg.vocab, device=ids.device, dtype=torch.float32) if return_logits else None
-        check(self.ctx, lib().tb_decoder_prefill(self._h, ctypes.c_void_p(ids.data_ptr()), ctypes.c_int(B),
-                                                 ctypes.c_int(S), ctypes.c_void_p(0 if logits is None else logits.data_ptr()),
-                                                 ctypes.c_void_p(nxt.data_ptr())))
+        with _on(self.device) as ctx:
+            check(ctx, lib().tb_decoder_prefill(self._h, ctypes.c_void_p(ids.data_ptr()), ctypes.c_int(B),
+                                                ctypes.c_int(S), ctypes.c_void_p(0 if logits is None else logits.data_ptr()),
+                                                ctypes.c_void_p(nxt.data_ptr())))
         self.B = B
         return (nxt, logits) if return_logits else nxt
 
     def decode_step(self, ids: torch.Tensor | None = None, return_logits: bool = False):
-        self._ctx()
         dev = torch.device("cuda", self.device)
         nxt = torch.empty(self.B, device=dev, dtype=torch.int32)
         logits = torch.empty(self.B, self.cfg.vocab, device=dev, dtype=torch.float32) if return_logits else None
         if ids is not None:
             ids = ids.to(torch.int32).contiguous()
-        check(self.ctx, lib().tb_decoder_decode_step(self._h, ctypes.c_void_p(0 if ids is None else ids.data_ptr()),
-                                                     ctypes.c_void_p(0 if logits is None else logits.data_ptr()),
-                                                     ctypes.c_void_p(nxt.data_ptr())))
+        with _on(self.device) as ctx:
+            check(ctx, lib().tb_decoder_decode_step(self._h, ctypes.c_void_p(0 if ids is None else ids.data_ptr()),
+                                                    ctypes.c_void_p(0 if logits is None else logits.data_ptr()),
+                                                    ctypes.c_void_p(nxt.data_ptr())))
         return (nxt, logits) if return_logits else nxt
 
     def generate(self, prompt_ids: torch.Tensor, n_new: int, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -162,9 +160,9 @@ class Decoder:
         B, S = prompt_ids.shape
         if out is None:
             out = torch.empty(B, n_new, device=prompt_ids.device, dtype=torch.int32)
-        self._ctx()
-        check(self.ctx, lib().tb_decoder_generate(self._h, ctypes.c_void_p(prompt_ids.data_ptr()), ctypes.c_int(B),
-                                                  ctypes.c_int(S), ctypes.c_int(n_new), ctypes.c_void_p(out.data_ptr())))
+        with _on(self.device) as ctx:
+            check(ctx, lib().tb_decoder_generate(self._h, ctypes.c_void_p(prompt_ids.data_ptr()), ctypes.c_int(B),
+                                                 ctypes.c_int(S), ctypes.c_int(n_new), ctypes.c_void_p(out.data_ptr())))
         self.B = B
         return out
 
@@ -172,9 +170,9 @@ class Decoder:
         """Decode-only workloads: KV cache of len(ids) sequences pre-filled with
         `length` positions of N(0,1); ids [B] are the current tokens."""
         ids = ids.to(torch.int32).contiguous()
-        self._ctx()
-        check(self.ctx, lib().tb_decoder_fill_kv_random(self._h, ctypes.c_int(ids.numel()), ctypes.c_int(length),
-                                                        ctypes.c_uint64(seed), ctypes.c_void_p(ids.data_ptr())))
+        with _on(self.device) as ctx:
+            check(ctx, lib().tb_decoder_fill_kv_random(self._h, ctypes.c_int(ids.numel()), ctypes.c_int(length),
+                                                       ctypes.c_uint64(seed), ctypes.c_void_p(ids.data_ptr())))
         self.B = ids.numel()
 
     def read_kv(self, layer: int, batch: int, length: int):
@@ -184,16 +182,17 @@ class Decoder:
         dev = torch.device("cuda", self.device)
         k = torch.empty(batch, c.n_kv_heads, length, c.head_dim, device=dev, dtype=torch.bfloat16)
         v = torch.empty_like(k)
-        self._ctx()
-        check(self.ctx, lib().tb_decoder_read_kv(self._h, ctypes.c_int(layer), ctypes.c_int(batch),
-                                                 ctypes.c_int(length), ctypes.c_void_p(k.data_ptr()),
-                                                 ctypes.c_void_p(v.data_ptr())))
+        with _on(self.device) as ctx:
+            check(ctx, lib().tb_decoder_read_kv(self._h, ctypes.c_int(layer), ctypes.c_int(batch),
+                                                ctypes.c_int(length), ctypes.c_void_p(k.data_ptr()),
+                                                ctypes.c_void_p(v.data_ptr())))
         torch.cuda.current_stream(dev).synchronize()
         return k, v
 
     def seq_len(self) -> int:
         n = ctypes.c_int(0)
-        check(self.ctx, lib().tb_decoder_seq_len(self._h, ctypes.byref(n)))
+        with _on(self.device) as ctx:
+            check(ctx, lib().tb_decoder_seq_len(self._h, ctypes.byref(n)))
         return n.value
 
 

@@ -12,7 +12,7 @@ import ctypes
 import torch
 
 from ._lib import TeenyError, check, lib
-from .ops import context
+from .ops import _on
 
 
 def shard(n: int, world: int, rank: int) -> tuple[int, int]:
@@ -52,9 +52,10 @@ class Comm:
         import torch.distributed as dist
         self.rank, self.world = rank, world
         self.device = torch.cuda.current_device() if device is None else device
-        self.ctx = context(self.device)
         uid = exchange_unique_id(nccl_unique_id, lambda t, src: self._bcast(dist, t, src), rank)
-        check(self.ctx, lib().tb_comm_init(self.ctx, ctypes.c_char_p(uid), ctypes.c_int(world), ctypes.c_int(rank),
+        with _on(self.device) as ctx:
+            self.ctx = ctx
+            check(ctx, lib().tb_comm_init(ctx, ctypes.c_char_p(uid), ctypes.c_int(world), ctypes.c_int(rank),
                                           ctypes.c_int(timeout_ms)))
 
     @staticmethod
@@ -71,10 +72,11 @@ class Comm:
         if out is None:
             out = torch.empty((self.world * local.shape[0],) + tuple(local.shape[1:]), dtype=local.dtype,
                               device=local.device)
-        ctx = context(self.device)
-        check(ctx, lib().tb_comm_allgather(ctx, ctypes.c_void_p(local.data_ptr()), ctypes.c_void_p(out.data_ptr()),
-                                           ctypes.c_size_t(local.numel() * local.element_size())))
+        with _on(self.device) as ctx:
+            check(ctx, lib().tb_comm_allgather(ctx, ctypes.c_void_p(local.data_ptr()), ctypes.c_void_p(out.data_ptr()),
+                                               ctypes.c_size_t(local.numel() * local.element_size())))
         return out
 
     def close(self):
-        lib().tb_comm_destroy(self.ctx)
+        with _on(self.device) as ctx:
+            lib().tb_comm_destroy(ctx)

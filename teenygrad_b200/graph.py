@@ -30,7 +30,7 @@ import ctypes
 import torch
 
 from ._lib import TB_ACT, TB_BF16, TB_F32, TB_I32, TeenyError, check, lib
-from .ops import context
+from .ops import _on
 
 _DT = {torch.float32: TB_F32, torch.bfloat16: TB_BF16, torch.int32: TB_I32}
 _TD = {v: k for k, v in _DT.items()}
@@ -161,7 +161,11 @@ class Graph:
 
     def compile(self, capture: bool = True):
         """Lowers the recorded ops onto tb_graph nodes and plans the arena."""
-        ctx = context(self.device)
+        with _on(self.device) as ctx:
+            self._lower(ctx, capture)
+        return self
+
+    def _lower(self, ctx, capture):
         l = lib()
         h = ctypes.c_void_p()
         check(ctx, l.tb_graph_create(ctx, ctypes.byref(h)))
@@ -244,7 +248,6 @@ class Graph:
             check(ctx, l.tb_graph_mark_output(h, ctypes.c_int(tid[o.idx])))
         check(ctx, l.tb_graph_plan(h, ctypes.c_int(int(capture))))
         self._tid = tid
-        return self
 
     def arena_bytes(self) -> int:
         n = ctypes.c_size_t(0)
@@ -257,25 +260,25 @@ class Graph:
         device tensors holding the outputs."""
         if self._h is None:
             raise TeenyError(1, "compile() first")
-        ctx = context(self.device)
         l = lib()
-        for v, t in zip(self.inputs, inputs):
-            t = t.to(v.dtype).contiguous()
-            check(ctx, l.tb_graph_write(self._h, ctypes.c_int(self._tid[v.idx]), ctypes.c_void_p(t.data_ptr()),
-                                        ctypes.c_size_t(t.numel() * t.element_size())))
-        check(ctx, l.tb_graph_run(self._h))
-        outs = []
-        for v in self.outputs:
-            o = torch.empty(v.shape, dtype=v.dtype, device=torch.device("cuda", self.device))
-            check(ctx, l.tb_graph_read(self._h, ctypes.c_int(self._tid[v.idx]), ctypes.c_void_p(o.data_ptr()),
-                                       ctypes.c_size_t(o.numel() * o.element_size())))
-            outs.append(o)
+        with _on(self.device) as ctx:
+            for v, t in zip(self.inputs, inputs):
+                t = t.to(v.dtype).contiguous()
+                check(ctx, l.tb_graph_write(self._h, ctypes.c_int(self._tid[v.idx]), ctypes.c_void_p(t.data_ptr()),
+                                            ctypes.c_size_t(t.numel() * t.element_size())))
+            check(ctx, l.tb_graph_run(self._h))
+            outs = []
+            for v in self.outputs:
+                o = torch.empty(v.shape, dtype=v.dtype, device=torch.device("cuda", self.device))
+                check(ctx, l.tb_graph_read(self._h, ctypes.c_int(self._tid[v.idx]), ctypes.c_void_p(o.data_ptr()),
+                                           ctypes.c_size_t(o.numel() * o.element_size())))
+                outs.append(o)
         return outs
 
     def launch(self):
         """The node launches only (inputs already written), on the current stream."""
-        ctx = context(self.device)
-        check(ctx, lib().tb_graph_run(self._h))
+        with _on(self.device) as ctx:
+            check(ctx, lib().tb_graph_run(self._h))
 
     def close(self):
         if self._h is not None:

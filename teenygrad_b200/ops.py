@@ -25,27 +25,35 @@ from ._lib import (TB_ACT, TB_BF16, TB_EPI_BIAS, TB_EPI_OUT_F32, TB_EPI_RESIDUAL
 
 _DT = {torch.float32: TB_F32, torch.bfloat16: TB_BF16}
 _ctxs: dict[int, ctypes.c_void_p] = {}
+_locks: dict[int, threading.RLock] = {}   # one for each device's context
+
+
+def _lock(device):
+    return _locks.get(device) or _locks.setdefault(device, threading.RLock())
 
 
 def context(device: int | None = None) -> ctypes.c_void_p:
-    """Per-device tb_ctx, bound to torch's current stream at each call."""
+    """Per-device tb_ctx, bound to torch's current stream at each call.  The operators share it, each for as
+    long as a call of the library takes (_on): code that makes its own calls with it must not do so while
+    other threads use the device's operators."""
     if device is None:
         device = torch.cuda.current_device()
-    ctx = _ctxs.get(device)
-    if ctx is None:
-        ctx = ctypes.c_void_p()
-        st = lib().tb_init(ctypes.byref(ctx), ctypes.c_int(device))
-        if st != 0:
-            raise TeenyError(st, f"tb_init(device={device}) failed: needs an sm_100 GPU")
-        _ctxs[device] = ctx
-    lib().tb_set_stream(ctx, ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream))
+    with _lock(device):
+        ctx = _ctxs.get(device)
+        if ctx is None:
+            ctx = ctypes.c_void_p()
+            st = lib().tb_init(ctypes.byref(ctx), ctypes.c_int(device))
+            if st != 0:
+                raise TeenyError(st, f"tb_init(device={device}) failed: needs an sm_100 GPU")
+            _ctxs[device] = ctx
+        lib().tb_set_stream(ctx, ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream))
     return ctx
 
 
 def device_error(clear: bool = True) -> int:
-    ctx = context()
     code = ctypes.c_int(0)
-    check(ctx, lib().tb_device_error(ctx, ctypes.byref(code), ctypes.c_int(int(clear))))
+    with _on() as ctx:
+        check(ctx, lib().tb_device_error(ctx, ctypes.byref(code), ctypes.c_int(int(clear))))
     return code.value
 
 
@@ -72,22 +80,22 @@ _i64 = ctypes.c_int64
 _f = ctypes.c_float
 
 
-_context_lock = threading.Lock()
-
-
 class _on:
-    """The context of a device, which is the current one inside the block.  The context's stream is the
-    calling thread's until the block ends: another thread that enters one waits (operators that use context()
-    alone do not)."""
+    """The context of a device (default: the current one), which is the current one inside the block.  A context
+    has one stream, one error text and one mode of launching, which are the calling thread's until the block ends:
+    another thread that enters one waits.  Every call that takes the context is made in such a block."""
 
-    __slots__ = ("device", "back")
+    __slots__ = ("device", "back", "lock")
 
-    def __init__(self, device):
+    def __init__(self, device=None):
         self.device = device
 
     def __enter__(self):
         self.back = torch.cuda.current_device()
-        _context_lock.acquire()
+        if self.device is None:
+            self.device = self.back
+        self.lock = _lock(self.device)
+        self.lock.acquire()
         try:
             if self.back != self.device:
                 torch.cuda.set_device(self.device)
@@ -101,7 +109,7 @@ class _on:
             raise
 
     def __exit__(self, *exc):
-        _context_lock.release()
+        self.lock.release()
         if self.back != self.device:
             torch.cuda.set_device(self.back)
 
@@ -134,8 +142,8 @@ def rms_norm(x, w, eps=1e-8, return_rrms=False):
     M = x.numel() // N
     y = torch.empty_like(x)
     rrms = torch.empty(M, device=x.device, dtype=torch.float32) if return_rrms else None
-    ctx = context()
-    check(ctx, lib().tb_rmsnorm_fwd(ctx, _dt(x), _p(x), _p(w), _p(y), _p(rrms), _i64(M), _i64(N), _f(eps)))
+    with _on() as ctx:
+        check(ctx, lib().tb_rmsnorm_fwd(ctx, _dt(x), _p(x), _p(w), _p(y), _p(rrms), _i64(M), _i64(N), _f(eps)))
     return (y, rrms) if return_rrms else y
 
 
@@ -158,8 +166,8 @@ def layer_norm(x, w, b, eps=1e-5, return_stats=False):
             check(ctx, lib().tb_layernorm_fwd_train(ctx, _dt(x), x.data_ptr(), w.data_ptr(), b.data_ptr(), y.data_ptr(),
                                                     mean.data_ptr(), rstd.data_ptr(), M, N, eps))
         return y, mean, rstd
-    ctx = context()
-    check(ctx, lib().tb_layernorm_fwd(ctx, _dt(x), _p(x), _p(w), _p(b), _p(y), _i64(x.numel() // N), _i64(N), _f(eps)))
+    with _on() as ctx:
+        check(ctx, lib().tb_layernorm_fwd(ctx, _dt(x), _p(x), _p(w), _p(b), _p(y), _i64(x.numel() // N), _i64(N), _f(eps)))
     return y
 
 
@@ -167,8 +175,8 @@ def layer_norm(x, w, b, eps=1e-5, return_stats=False):
 def activation(kind, x):
     _cuda(x)
     y = torch.empty_like(x)
-    ctx = context()
-    check(ctx, lib().tb_act_fwd(ctx, ctypes.c_int(TB_ACT[kind]), _dt(x), _p(x), _p(y), _i64(x.numel())))
+    with _on() as ctx:
+        check(ctx, lib().tb_act_fwd(ctx, ctypes.c_int(TB_ACT[kind]), _dt(x), _p(x), _p(y), _i64(x.numel())))
     return y
 
 
@@ -191,16 +199,16 @@ def sigmoid(x):
 def swiglu(gate, up):
     _cuda(gate, up)
     y = torch.empty_like(gate)
-    ctx = context()
-    check(ctx, lib().tb_swiglu_fwd(ctx, _dt(gate), _p(gate), _p(up), _p(y), _i64(gate.numel())))
+    with _on() as ctx:
+        check(ctx, lib().tb_swiglu_fwd(ctx, _dt(gate), _p(gate), _p(up), _p(y), _i64(gate.numel())))
     return y
 
 
 def add(a, b):
     _cuda(a, b)
     y = torch.empty_like(a)
-    ctx = context()
-    check(ctx, lib().tb_add_fwd(ctx, _dt(a), _p(a), _p(b), _p(y), _i64(a.numel())))
+    with _on() as ctx:
+        check(ctx, lib().tb_add_fwd(ctx, _dt(a), _p(a), _p(b), _p(y), _i64(a.numel())))
     return y
 
 
@@ -220,9 +228,9 @@ def linear(x, w, bias=None, residual=None, swiglu=False, out_f32=False):
     y = torch.empty(*x.shape[:-1], ncol, device=x.device, dtype=torch.float32 if out_f32 else x.dtype)
     if bias is not None and bias.dtype != torch.float32:
         bias = bias.float().contiguous()
-    ctx = context()
-    check(ctx, lib().tb_linear_fwd(ctx, _dt(x), _p(x), _p(w), _p(bias), _p(residual), _p(y),
-                                   _i64(M), _i64(N), _i64(K), ctypes.c_int(flags)))
+    with _on() as ctx:
+        check(ctx, lib().tb_linear_fwd(ctx, _dt(x), _p(x), _p(w), _p(bias), _p(residual), _p(y),
+                                       _i64(M), _i64(N), _i64(K), ctypes.c_int(flags)))
     return y
 
 
@@ -255,8 +263,8 @@ def linear_chain(steps):
         arr[i] = _LinearStep(addr(x), x.stride(-2) if x.dim() > 1 else K, addr(w), addr(st.get("norm_w")),
                              float(st.get("eps", 1e-5)), addr(st.get("residual")), addr(y),
                              y.stride(-2) if y.dim() > 1 else y.shape[-1], w.shape[0], K, flags)
-    ctx = context()
-    check(ctx, lib().tb_linear_chain_fwd(ctx, arr, ctypes.c_int(len(steps)), _i64(M)))
+    with _on() as ctx:
+        check(ctx, lib().tb_linear_chain_fwd(ctx, arr, ctypes.c_int(len(steps)), _i64(M)))
 
 
 TB_OP = {"linear": 0, "matmul": 1, "int8_linear": 2, "rmsnorm": 3, "layernorm": 4, "act": 5, "attn": 6,
@@ -284,10 +292,10 @@ def linear_padded(x, w, bias=None):
     buf = torch.full((M, ld), float("nan"), device=x.device, dtype=x.dtype)
     if bias is not None and bias.dtype != torch.float32:
         bias = bias.float().contiguous()
-    ctx = context()
-    check(ctx, lib().tb_linear_fwd_strided(ctx, _dt(x), _p(x), _i64(K), _p(w), _p(bias), _p(None), _p(buf), _i64(ld),
-                                           _i64(M), _i64(N), _i64(K),
-                                           ctypes.c_int(TB_EPI_BIAS if bias is not None else 0)))
+    with _on() as ctx:
+        check(ctx, lib().tb_linear_fwd_strided(ctx, _dt(x), _p(x), _i64(K), _p(w), _p(bias), _p(None), _p(buf), _i64(ld),
+                                               _i64(M), _i64(N), _i64(K),
+                                               ctypes.c_int(TB_EPI_BIAS if bias is not None else 0)))
     return buf, buf[:, :N]
 
 
@@ -306,8 +314,8 @@ def matmul(a, b):
     M, K = a.shape
     N = b.shape[1]
     c = torch.empty(M, N, device=a.device, dtype=a.dtype)
-    ctx = context()
-    check(ctx, lib().tb_matmul_fwd(ctx, _dt(a), _p(a), _p(b), _p(c), _i64(M), _i64(N), _i64(K)))
+    with _on() as ctx:
+        check(ctx, lib().tb_matmul_fwd(ctx, _dt(a), _p(a), _p(b), _p(c), _i64(M), _i64(N), _i64(K)))
     return c
 
 
@@ -318,9 +326,9 @@ def quantize_int8(w):
     N, K = w.shape
     q = torch.empty(N, K, device=w.device, dtype=torch.int8)
     s = torch.empty(N, device=w.device, dtype=torch.float32)
-    ctx = context()
     fn = lib().tb_quantize_int8 if w.dtype == torch.float32 else lib().tb_quantize_int8_bf16
-    check(ctx, fn(ctx, _p(w), _p(q), _p(s), _i64(N), _i64(K)))
+    with _on() as ctx:
+        check(ctx, fn(ctx, _p(w), _p(q), _p(s), _i64(N), _i64(K)))
     return q, s
 
 
@@ -328,8 +336,8 @@ def dequantize_int8(q, s):
     _cuda(q, s)
     N, K = q.shape
     w = torch.empty(N, K, device=q.device, dtype=torch.float32)
-    ctx = context()
-    check(ctx, lib().tb_dequantize_int8(ctx, _p(q), _p(s), _p(w), _i64(N), _i64(K)))
+    with _on() as ctx:
+        check(ctx, lib().tb_dequantize_int8(ctx, _p(q), _p(s), _p(w), _i64(N), _i64(K)))
     return w
 
 
@@ -342,9 +350,9 @@ def int8_linear(x, q, s, residual=None, swiglu=False, out_f32=False):
     flags |= TB_EPI_OUT_F32 if out_f32 else 0
     ncol = N // 2 if swiglu else N
     y = torch.empty(*x.shape[:-1], ncol, device=x.device, dtype=torch.float32 if out_f32 else x.dtype)
-    ctx = context()
-    check(ctx, lib().tb_int8_linear_fwd(ctx, _p(x), _p(q), _p(s), _p(residual), _p(y), _i64(M), _i64(N),
-                                        _i64(K), ctypes.c_int(flags)))
+    with _on() as ctx:
+        check(ctx, lib().tb_int8_linear_fwd(ctx, _p(x), _p(q), _p(s), _p(residual), _p(y), _i64(M), _i64(N),
+                                            _i64(K), ctypes.c_int(flags)))
     return y
 
 
@@ -359,10 +367,10 @@ def attention(q, k, v, scale=None, causal=False, return_lse=False):
         scale = 1.0 / math.sqrt(D)
     o = torch.empty_like(q)
     lse = torch.empty(B, Hq, Sq, device=q.device, dtype=torch.float32) if return_lse else None
-    ctx = context()
-    check(ctx, lib().tb_attn_fwd(ctx, _dt(q), _p(q), _p(k), _p(v), _p(o), _p(lse), ctypes.c_int(B),
-                                 ctypes.c_int(Hq), ctypes.c_int(Hkv), ctypes.c_int(Sq), ctypes.c_int(Sk),
-                                 ctypes.c_int(D), _f(scale), ctypes.c_int(int(causal))))
+    with _on() as ctx:
+        check(ctx, lib().tb_attn_fwd(ctx, _dt(q), _p(q), _p(k), _p(v), _p(o), _p(lse), ctypes.c_int(B),
+                                     ctypes.c_int(Hq), ctypes.c_int(Hkv), ctypes.c_int(Sq), ctypes.c_int(Sk),
+                                     ctypes.c_int(D), _f(scale), ctypes.c_int(int(causal))))
     return (o, lse) if return_lse else o
 
 
@@ -372,8 +380,8 @@ def rope(x, pos, theta=10000.0):
     _cuda(x, pos)
     T, H, D = x.shape
     y = torch.empty_like(x)
-    ctx = context()
-    check(ctx, lib().tb_rope_fwd(ctx, _dt(x), _p(x), _p(pos), _p(y), _i64(T), ctypes.c_int(H), ctypes.c_int(D), _f(theta)))
+    with _on() as ctx:
+        check(ctx, lib().tb_rope_fwd(ctx, _dt(x), _p(x), _p(pos), _p(y), _i64(T), ctypes.c_int(H), ctypes.c_int(D), _f(theta)))
     return y
 
 
@@ -382,8 +390,8 @@ def embedding(table, ids):
     T = ids.numel()
     D = table.shape[1]
     y = torch.empty(T, D, device=table.device, dtype=table.dtype)
-    ctx = context()
-    check(ctx, lib().tb_embedding_fwd(ctx, _dt(table), _p(table), _p(ids), _p(y), _i64(T), _i64(D), _i64(table.shape[0])))
+    with _on() as ctx:
+        check(ctx, lib().tb_embedding_fwd(ctx, _dt(table), _p(table), _p(ids), _p(y), _i64(T), _i64(D), _i64(table.shape[0])))
     return y
 
 
@@ -391,8 +399,8 @@ def argmax(x):
     _cuda(x)
     M, N = x.shape
     out = torch.empty(M, device=x.device, dtype=torch.int32)
-    ctx = context()
-    check(ctx, lib().tb_argmax_fwd(ctx, _dt(x), _p(x), _p(out), _i64(M), _i64(N)))
+    with _on() as ctx:
+        check(ctx, lib().tb_argmax_fwd(ctx, _dt(x), _p(x), _p(out), _i64(M), _i64(N)))
     return out
 
 
@@ -446,9 +454,9 @@ def bn_fold(gamma, beta, mean, var, eps=1e-5, bias=None):
     C = gamma.numel()
     scale = torch.empty(C, device=gamma.device, dtype=torch.float32)
     shift = torch.empty_like(scale)
-    ctx = context()
-    check(ctx, lib().tb_bn_fold(ctx, _p(gamma), _p(beta), _p(mean), _p(var), _p(bias), _f(eps), _p(scale), _p(shift),
-                                ctypes.c_int(C)))
+    with _on() as ctx:
+        check(ctx, lib().tb_bn_fold(ctx, _p(gamma), _p(beta), _p(mean), _p(var), _p(bias), _f(eps), _p(scale), _p(shift),
+                                    ctypes.c_int(C)))
     return scale, shift
 
 
@@ -458,9 +466,9 @@ def batch_norm_inference(x, gamma, beta, mean, var, eps=1e-5):
     B, C = x.shape[0], x.shape[1]
     HW = x.numel() // max(1, B * C)
     y = torch.empty_like(x)
-    ctx = context()
-    check(ctx, lib().tb_batchnorm_fwd(ctx, _dt(x), _p(x), _p(gamma), _p(beta), _p(mean), _p(var), _p(y), _i64(B),
-                                      _i64(C), _i64(HW), _f(eps)))
+    with _on() as ctx:
+        check(ctx, lib().tb_batchnorm_fwd(ctx, _dt(x), _p(x), _p(gamma), _p(beta), _p(mean), _p(var), _p(y), _i64(B),
+                                          _i64(C), _i64(HW), _f(eps)))
     return y
 
 
@@ -496,12 +504,12 @@ def conv2d(x, w, bias=None, scale=None, shift=None, stride=1, pad=0, act=None, x
                                             ctypes.byref(nbytes))
         check(None, st)
     ws = torch.empty(max(1, nbytes.value), device=x.device, dtype=torch.uint8) if nbytes.value else None
-    ctx = context()
     f = [t if t is None or t.dtype == torch.float32 else t.float().contiguous() for t in (bias, scale, shift)]
-    check(ctx, lib().tb_conv2d_fwd_ex(ctx, ctypes.c_int(_dt(x)), _p(x), _p(w), _p(f[0]), _p(f[1]), _p(f[2]), _p(y),
-                                      *(ctypes.c_int(v) for v in (B, C, Co, H, W, KH, KW, stride, pad, _CONV_ACT[act],
-                                                                   flags)),
-                                      _p(ws), ctypes.c_size_t(nbytes.value)))
+    with _on() as ctx:
+        check(ctx, lib().tb_conv2d_fwd_ex(ctx, ctypes.c_int(_dt(x)), _p(x), _p(w), _p(f[0]), _p(f[1]), _p(f[2]), _p(y),
+                                          *(ctypes.c_int(v) for v in (B, C, Co, H, W, KH, KW, stride, pad, _CONV_ACT[act],
+                                                                       flags)),
+                                          _p(ws), ctypes.c_size_t(nbytes.value)))
     return y
 
 
@@ -510,9 +518,9 @@ def conv2d_pack_weights(w):
     _cuda(w)
     Co, C, KH, KW = w.shape
     out = torch.empty(Co, KH, KW, C, device=w.device, dtype=w.dtype)
-    ctx = context()
-    check(ctx, lib().tb_conv2d_pack_weights(ctx, ctypes.c_int(_dt(w)), _p(w), _p(out),
-                                            *(ctypes.c_int(v) for v in (Co, C, KH, KW))))
+    with _on() as ctx:
+        check(ctx, lib().tb_conv2d_pack_weights(ctx, ctypes.c_int(_dt(w)), _p(w), _p(out),
+                                                *(ctypes.c_int(v) for v in (Co, C, KH, KW))))
     return out
 
 
@@ -551,9 +559,9 @@ def rms_norm_backward(dy, x, w, rrms, dw=None):
     if dw is None:
         dw = torch.zeros(N, device=x.device, dtype=torch.float32)
     ws, nb = _workspace("rmsnorm_bwd", _dt(x), (M, N), x.device)
-    ctx = context()
-    check(ctx, lib().tb_rmsnorm_bwd(ctx, _dt(x), _p(dy), _p(x), _p(w), _p(rrms), _p(dx), _p(dw), _i64(M), _i64(N),
-                                    _p(ws), ctypes.c_size_t(nb)))
+    with _on() as ctx:
+        check(ctx, lib().tb_rmsnorm_bwd(ctx, _dt(x), _p(dy), _p(x), _p(w), _p(rrms), _p(dx), _p(dw), _i64(M), _i64(N),
+                                        _p(ws), ctypes.c_size_t(nb)))
     return dx, dw
 
 
@@ -596,9 +604,9 @@ def linear_backward(x, w, dy, bias=True):
     dw = torch.empty_like(w)
     db = torch.empty(N, device=x.device, dtype=torch.float32) if bias else None
     ws, nb = _workspace("linear_bwd", _dt(x), (M, N, K), x.device)
-    ctx = context()
-    check(ctx, lib().tb_linear_bwd(ctx, _dt(x), _p(x), _p(w), _p(dy), _p(dx), _p(dw), _p(db), _i64(M), _i64(N),
-                                   _i64(K), _p(ws), ctypes.c_size_t(nb)))
+    with _on() as ctx:
+        check(ctx, lib().tb_linear_bwd(ctx, _dt(x), _p(x), _p(w), _p(dy), _p(dx), _p(dw), _p(db), _i64(M), _i64(N),
+                                       _i64(K), _p(ws), ctypes.c_size_t(nb)))
     return dx, dw, db
 
 
@@ -612,10 +620,10 @@ def attention_backward(q, k, v, o, do, lse, scale=None, causal=False):
         scale = 1.0 / math.sqrt(D)
     dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
     ws, nb = _workspace("attn_bwd", _dt(q), (B, Hq, Sq), q.device)
-    ctx = context()
-    check(ctx, lib().tb_attn_bwd(ctx, _dt(q), _p(q), _p(k), _p(v), _p(o), _p(do), _p(lse), _p(dq), _p(dk), _p(dv),
-                                 ctypes.c_int(B), ctypes.c_int(Hq), ctypes.c_int(Hkv), ctypes.c_int(Sq), ctypes.c_int(Sk),
-                                 ctypes.c_int(D), _f(scale), ctypes.c_int(int(causal)), _p(ws), ctypes.c_size_t(nb)))
+    with _on() as ctx:
+        check(ctx, lib().tb_attn_bwd(ctx, _dt(q), _p(q), _p(k), _p(v), _p(o), _p(do), _p(lse), _p(dq), _p(dk), _p(dv),
+                                     ctypes.c_int(B), ctypes.c_int(Hq), ctypes.c_int(Hkv), ctypes.c_int(Sq), ctypes.c_int(Sk),
+                                     ctypes.c_int(D), _f(scale), ctypes.c_int(int(causal)), _p(ws), ctypes.c_size_t(nb)))
     return dq, dk, dv
 
 
@@ -625,10 +633,10 @@ def conv2d_backward(dy, x, w, stride=1, pad=0):
     B, Cin, H, W = x.shape
     Cout, _, KH, KW = w.shape
     dx, dw = torch.empty_like(x), torch.empty_like(w)
-    ctx = context()
-    check(ctx, lib().tb_conv2d_bwd(ctx, _dt(x), _p(dy), _p(x), _p(w), _p(dx), _p(dw), ctypes.c_int(B),
-                                   ctypes.c_int(Cin), ctypes.c_int(Cout), ctypes.c_int(H), ctypes.c_int(W),
-                                   ctypes.c_int(KH), ctypes.c_int(KW), ctypes.c_int(stride), ctypes.c_int(pad)))
+    with _on() as ctx:
+        check(ctx, lib().tb_conv2d_bwd(ctx, _dt(x), _p(dy), _p(x), _p(w), _p(dx), _p(dw), ctypes.c_int(B),
+                                       ctypes.c_int(Cin), ctypes.c_int(Cout), ctypes.c_int(H), ctypes.c_int(W),
+                                       ctypes.c_int(KH), ctypes.c_int(KW), ctypes.c_int(stride), ctypes.c_int(pad)))
     return dx, dw
 
 
