@@ -155,6 +155,8 @@ __device__ __forceinline__ void store4(T* p, int64_t i, int64_t n, bool vec, con
 // The step's scalars.
 struct Step {
     float scale, keep, rate, root, eps;   // keep = 1 - lr wd, rate = lr / (1 - b1^t), root = 1 / sqrt(1 - b2^t)
+    // A root that the hardware's flushes to 0 is under 2^-63: times `root`, under 2^-24 of an eps above this.
+    float flushed;
     uint32_t key;
 };
 
@@ -180,6 +182,7 @@ __device__ __forceinline__ Step step_of(const Hyper& h) {
     s.rate = lr / -expm1f((float)t * h.log1);
     s.root = rsqrtf(-expm1f((float)t * h.log2));
     s.eps = h.eps;
+    s.flushed = fmaxf(0x1p-39f * s.root, 1e-30f);
     s.key = mix(mix(h.seed) ^ (uint32_t)t);
     return s;
 }
@@ -417,7 +420,8 @@ __device__ __forceinline__ void fetch(UnitIn<P, G>& in, const Entry& e, int unit
 // The two blocks of a whole unit at aligned addresses; false, with nothing written, where one is
 // not a common one.  The common case folds the exponents into the betas (exact, as they are powers
 // of two) and takes the hardware's square root (2^-23), which flushes what is under 2^-126: no code
-// depends on its last places there, and the step does only where eps is as small as such a root.
+// depends on its last places there, and the step does only where eps is as small as such a root
+// (Step::flushed).
 // exps: m's exponents in bytes 0 and 1, s's in 2 and 3.
 template <typename P, typename G>
 __device__ __forceinline__ bool adamw8_unit(const UnitIn<P, G>& in, uint32_t exps, const Entry& e, int unit, const Hyper& h,
@@ -427,10 +431,7 @@ __device__ __forceinline__ bool adamw8_unit(const UnitIn<P, G>& in, uint32_t exp
     const F2 scale2 = f2(s.scale, s.scale), r1 = f2(h.rest1, h.rest1), r2 = f2(h.rest2, h.rest2);
     float m[8 * B], v[8 * B];
     uint32_t tm[B], tv[B];
-    // A flushed root is under 2^-63: next to an eps above 2^-39 root it is under 2^-24 of the divisor.  Where eps is
-    // smaller, blocks that hold one are not common ones, and eps itself is above what the reciprocal flushes.
-    const bool flushed_counts = !(s.eps > 0x1p-39f * s.root);
-    bool common = s.eps > 1e-30f, any_flushed = false;
+    bool common = true;
 #pragma unroll
     for (int b = 0; b < B; b++) {
         // m beta1 = code * bm and s^2 beta2 = code^2 * bs
@@ -458,9 +459,6 @@ __device__ __forceinline__ bool adamw8_unit(const UnitIn<P, G>& in, uint32_t exp
                 top_v = largest(top_v, v[k], v[k + 1]);
             }
         }
-        if (flushed_counts)
-#pragma unroll
-            for (int k = 8 * b; k < 8 * b + 8; k++) any_flushed |= v[k] > 0.f && v[k] < 0x1p-126f;
         tm[b] = __reduce_max_sync(0xffffffffu, __float_as_uint(top_m));
         tv[b] = __reduce_max_sync(0xffffffffu, __float_as_uint(top_v));
         // Moments under 2^14, so that the scale below is a normal number (what is not finite is above); a largest
@@ -469,8 +467,13 @@ __device__ __forceinline__ bool adamw8_unit(const UnitIn<P, G>& in, uint32_t exp
         common = common && tm[b] < 141u << 23 && tv[b] < 155u << 23 && (tv[b] >= 43u << 23 || tv[b] == 0) &&
                  ((em >= 32 && es >= 84) || __all_sync(0xffffffffu, !codes));
     }
-    if (flushed_counts) common = common && !__any_sync(0xffffffffu, any_flushed);
     if (!common) return false;
+    if (s.eps <= s.flushed) {
+        bool any = s.eps <= 1e-30f;   // what the reciprocal flushes
+#pragma unroll
+        for (int k = 0; k < 8 * B; k++) any |= v[k] > 0.f && v[k] < 0x1p-126f;
+        if (__any_sync(0xffffffffu, any)) return false;
+    }
     const F2 root2 = f2(s.root, s.root), eps2 = f2(s.eps, s.eps), rate2 = f2(-s.rate, -s.rate), keep2 = f2(s.keep, s.keep);
     const int64_t i0 = (int64_t)unit * kUnit8 + at;
     const uint32_t hash = hash_of(key, i0);
