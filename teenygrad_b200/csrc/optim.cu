@@ -31,6 +31,7 @@
 // issue comes first, 56 of them an element.  1.1e9 bf16 gradients' norm 0.32 ms.
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
+#include <float.h>
 #include <math.h>
 #include <stdlib.h>
 
@@ -868,7 +869,9 @@ int tb_adamw_step(tb_adamw* a, const tb_adamw_hyper* hy) {
     h.beta2 = (float)hy->beta2;
     h.rest1 = (float)(1.0 - hy->beta1);
     h.rest2 = (float)(1.0 - hy->beta2);
-    h.eps = (float)hy->eps;
+    // The division flushes a divisor under 2^-126, so an eps above 0 is at least that: 0 / eps stays 0, and next to a
+    // root above 0 (2^-75 at least, that of f32's smallest number) neither is seen.
+    h.eps = hy->eps > 0 ? std::max((float)hy->eps, FLT_MIN) : 0.f;
     h.decay = (float)hy->weight_decay;
     h.log1 = (float)log(hy->beta1);   // -inf for 0: the correction is 1
     h.log2 = (float)log(hy->beta2);

@@ -650,3 +650,25 @@ def test_adamw_8_bits_where_the_root_is_next_to_a_small_eps(pt, gt, copy, eps):
         m.check_codes(0, u.adamw8_moments(m.g[0], zero.astype(np.uint8), np.zeros(-(-n // 256), np.uint8), zero.astype(np.uint8),
                                           np.zeros(-(-n // 256), np.uint8), 0, t, 0, B1, B2, 1.0))
         m.p[0] = got
+
+
+@pytest.mark.parametrize("eps", [1e-37, 1e-40, 1e-50])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_with_an_eps_under_f32s_normal_numbers(bits, eps):
+    """What has no gradient and no moments is only decayed, for as long as eps is not 0."""
+    ops()
+    m = Model([1000], F32, F32, False, bits, seed=42)
+    none = np.arange(1000) % 3 == 0
+    m.g[0][none] = 0
+    m.grads[0].copy_(torch.from_numpy(m.g[0]))
+    if bits == 32:
+        for held, name in ((m.m, "m"), (m.v, "v")):
+            held[0][none] = 0
+            m.state[name][0].copy_(torch.from_numpy(held[0]))
+    else:
+        for held, name in ((m.m, "m"), (m.s, "s")):
+            held[0][0][none] = 0
+            m.codes[name][0].copy_(torch.from_numpy(held[0][0]))
+    o = m.optimiser(eps=eps, step_count=4)
+    o.step()
+    m.check(5, eps=eps)
