@@ -305,9 +305,9 @@ TB_API int tb_conv2d_bwd(tb_ctx* ctx, int dtype, const void* dy, const void* x, 
 /* The 2-norm of all the elements of n gradient tensors (device pointers and
  * sizes in host arrays; dtype TB_F32 or TB_BF16): norm[0] (f32, device), and, when
  * scale is given, scale[0] = min(1, max_norm / (norm + 1e-6)), the factor that clips
- * the gradients to max_norm (NaN for a NaN norm).  Squares are f32: one above
- * 3.4e38 makes the norm infinite.  Sums in a fixed order.  Workspace:
- * TB_OP_GRAD_NORM {n}, 8-byte aligned. */
+ * the gradients to max_norm (NaN for a NaN norm).  Elements of any size count: the
+ * norm is infinite only where f32 does not hold it.  Sums in a fixed order.
+ * Workspace: TB_OP_GRAD_NORM {n}, 8-byte aligned. */
 TB_API int tb_grad_norm(tb_ctx* ctx, int dtype, const void* const* grads, const int64_t* sizes, int n, float* norm,
                         float* scale, double max_norm, void* workspace, size_t workspace_bytes);
 

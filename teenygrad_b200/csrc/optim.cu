@@ -613,20 +613,31 @@ __global__ void __launch_bounds__(kThreads8, Ring8<P, G>::ctas) adamw8_kernel(co
 }
 
 // -------------------------------------------------------------- grad norm --
-__device__ __forceinline__ float sumsq16(const uint4 a, const float*) {
-    const float x = __uint_as_float(a.x), y = __uint_as_float(a.y), z = __uint_as_float(a.z), w = __uint_as_float(a.w);
+// The sum of the squares of 16 bytes, each element times f.
+__device__ __forceinline__ float sumsq16(const uint4 a, const float*, float f = 1.f) {
+    const float x = __uint_as_float(a.x) * f, y = __uint_as_float(a.y) * f, z = __uint_as_float(a.z) * f,
+                w = __uint_as_float(a.w) * f;
     return (x * x + y * y) + (z * z + w * w);
 }
-__device__ __forceinline__ float sumsq16(const uint4 a, const bf16*) {
-    const float x = bf16_lo(a.x) * bf16_lo(a.x) + bf16_hi(a.x) * bf16_hi(a.x);
-    const float y = bf16_lo(a.y) * bf16_lo(a.y) + bf16_hi(a.y) * bf16_hi(a.y);
-    const float z = bf16_lo(a.z) * bf16_lo(a.z) + bf16_hi(a.z) * bf16_hi(a.z);
-    const float w = bf16_lo(a.w) * bf16_lo(a.w) + bf16_hi(a.w) * bf16_hi(a.w);
-    return (x + y) + (z + w);
+__device__ __forceinline__ float sumsq2(uint32_t a, float f) {
+    const float x = bf16_lo(a) * f, y = bf16_hi(a) * f;
+    return x * x + y * y;
 }
+__device__ __forceinline__ float sumsq16(const uint4 a, const bf16*, float f = 1.f) {
+    return (sumsq2(a.x, f) + sumsq2(a.y, f)) + (sumsq2(a.z, f) + sumsq2(a.w, f));
+}
+
+// Whether a thread's sum of squares leaves f32's range at either end: one under 2^-80 may have lost squares to it
+// (above that, those under 2^-126 are nothing), one that is not finite may be of finite elements.
+__device__ __forceinline__ bool out_of_range(float s) { return !(s > 0x1p-80f && s < INFINITY); }
+// What takes the elements of such a sum to where f32 holds their squares, exactly, as it is a power of two; the sum's
+// own factor is its square's inverse.
+__device__ __forceinline__ float range_factor(float s) { return s < 1.f ? 0x1p100f : 0x1p-100f; }
+__device__ __forceinline__ double from_range(float s, float f) { return (double)s * (f > 1.f ? 0x1p-200 : 0x1p200); }
 
 // part[blockIdx.x] = the CTA's sum of squares: f32 over a chunk's 32 elements a
 // thread, f64 over the chunks.  All of a chunk's loads are in flight at once.
+// Where f32 does not hold the squares, the elements are taken again, scaled.
 template <typename G, int CAP>
 __global__ void __launch_bounds__(kThreads) sumsq_kernel(const __grid_constant__ Table<CAP> t, double* __restrict__ part) {
     constexpr int V = 16 / sizeof(G), L = kNormChunk / kThreads / V;
@@ -645,11 +656,29 @@ __global__ void __launch_bounds__(kThreads) sumsq_kernel(const __grid_constant__
             for (int u = 0; u < L; u++) a[u] = *reinterpret_cast<const uint4*>(g + i0 + (u * kThreads + threadIdx.x) * V);
 #pragma unroll
             for (int u = 0; u < L; u++) s += sumsq16(a[u], g);
+            if (out_of_range(s)) {
+                const float f = range_factor(s);
+                s = 0.f;
+#pragma unroll
+                for (int u = 0; u < L; u++) s += sumsq16(a[u], g, f);
+                acc += from_range(s, f);
+                continue;
+            }
         } else {
 #pragma unroll 8
             for (int64_t i = i0 + threadIdx.x; i < n && i < i0 + kNormChunk; i += kThreads) {
                 const float x = load1(g + i);
                 s += x * x;
+            }
+            if (out_of_range(s)) {
+                const float f = range_factor(s);
+                s = 0.f;
+                for (int64_t i = i0 + threadIdx.x; i < n && i < i0 + kNormChunk; i += kThreads) {
+                    const float x = load1(g + i) * f;
+                    s += x * x;
+                }
+                acc += from_range(s, f);
+                continue;
             }
         }
         acc += s;

@@ -672,3 +672,21 @@ def test_adamw_with_an_eps_under_f32s_normal_numbers(bits, eps):
     o = m.optimiser(eps=eps, step_count=4)
     o.step()
     m.check(5, eps=eps)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("size", [1e-43, 1e-38, 1e-30, 1e-22, 1e-19, 1e-13, 1e12, 1e18, 1e25, 1e35])
+def test_grad_norm_of_sizes_whose_squares_f32_does_not_hold(dtype, size):
+    o, r = ops(), rng(7)
+    small = size < 1
+    # next to ordinary ones where those do not hide them: chunks of their own, and a few among zeros
+    g = [r.standard_normal(20000) * size, np.where(r.random(9000) < 0.01, r.standard_normal(9000) * size, 0.0), np.zeros(8192)]
+    if not small:
+        g.append(r.standard_normal(5000))
+    g = [rounded(a.astype(np.float32), dtype) for a in g]
+    ts = [place(a, dtype, odd=k % 2 == 1)[0] for k, a in enumerate(g)]
+    want = np.sqrt(sum(float((a.astype(np.float64) ** 2).sum()) for a in g))
+    norm, scale = o.grad_norm(ts, max_norm=1.0)
+    # as test_grad_norm has it; a result under 2^-126 has steps of 2^-149
+    assert abs(float(norm) - want) <= 18 * u.U32 * want + 2.0 ** -150
+    assert abs(float(scale) - min(1.0, 1 / (want + 1e-6))) <= 20 * u.U32 / max(want, 1.0)
