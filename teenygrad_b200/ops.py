@@ -85,7 +85,7 @@ class _on:
     has one stream, one error text and one mode of launching, which are the calling thread's until the block ends:
     another thread that enters one waits.  Every call that takes the context is made in such a block."""
 
-    __slots__ = ("device", "back", "lock")
+    __slots__ = ("device", "back", "lock", "stream")
 
     def __init__(self, device=None):
         self.device = device
@@ -99,10 +99,9 @@ class _on:
         try:
             if self.back != self.device:
                 torch.cuda.set_device(self.device)
-            ctx = _ctxs.get(self.device)
-            if ctx is None:
-                return context(self.device)
-            lib().tb_set_stream(ctx, torch._C._cuda_getCurrentRawStream(self.device))
+            ctx = _ctxs.get(self.device) or context(self.device)
+            self.stream = torch._C._cuda_getCurrentRawStream(self.device)
+            lib().tb_set_stream(ctx, self.stream)
             return ctx
         except BaseException:
             self.__exit__()
@@ -698,8 +697,9 @@ class AdamW:
         p = p (1 - lr weight_decay) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
 
     params and grads: lists of contiguous CUDA tensors, f32 / f32, f32 / bf16 or bf16 / bf16;
-    copies: bf16 tensors that get each step's f32 parameters.  The addresses are kept: step() refuses
-    to run once one of these has been given other memory.  Tensors must not overlap.
+    copies: bf16 tensors that get each step's f32 parameters.  Addresses are kept, the moments' too: step()
+    refuses to run once a tensor has been given other memory, or another one takes its place in a list.
+    Tensors must not overlap.
 
     state_bits=32: m and v are f32.  state_bits=8: m and s = sqrt(v) are float8_e4m3fn with a uint8
     exponent for each 256 elements (m_exp, s_exp): code * 2^(exp - 127), rounded up or down at random
@@ -752,15 +752,14 @@ class AdamW:
                 raise TeenyError(5, f"copies must be bfloat16, got {cd}")
         if n and (pd not in _DT or gd not in _DT):
             raise TeenyError(5, f"unsupported dtypes {pd}, {gd}")
-        lists = [self.params, self.grads, self.copies or []] + [getattr(self, name) for name, _, _ in names]
+        self._lists = ("params", "grads") + (() if self.copies is None else ("copies",)) + tuple(name for name, _, _ in names)
         if n and len(devices) > 1:
             raise TeenyError(1, "tensors must be on one device")
         exps = ptrs[2:] or [[0] * n, [0] * n]
         rows = array.array("Q", [f for row in zip(pp, gp, ptrs[0], ptrs[1], *exps, cp, sizes) for f in row])
         # the memory lives as long as the optimiser, whatever becomes of the tensors
-        self._alive = [t.detach() for ts in lists for t in ts]
-        self._watched = [t for ts in lists[:3] for t in ts]
-        self._at = list(map(_T.data_ptr, self._watched))
+        self._alive = [t.detach() for name in self._lists for t in getattr(self, name)]
+        self._at = self._addresses()
         self._hyper = _AdamWHyper(0.0, betas[0], betas[1], eps, weight_decay, 0, seed & 0xFFFFFFFF, None, None, None)
         self._step_dev, self._step = None, step_count
         self._captured = []   # scalars that captured steps read at each replay
@@ -787,8 +786,14 @@ class AdamW:
         """Steps taken (waits for the device when capturable)."""
         return self._step if self._step_dev is None else int(self._step_dev)
 
+    def _addresses(self):
+        at = []
+        for name in self._lists:
+            at += map(_T.data_ptr, getattr(self, name))
+        return at
+
     def _scalar(self, what, t):
-        if not t.is_cuda or t.dtype != torch.float32 or t.numel() != 1 or t.get_device() != self.device:
+        if t.get_device() != self.device or t.dtype != torch.float32 or t.numel() != 1:
             raise TeenyError(1, f"{what}: an f32 tensor of one element on the parameters' device")
         return t.data_ptr()
 
@@ -797,8 +802,8 @@ class AdamW:
         self.lr).  grad_scale: such a tensor, which multiplies the gradients."""
         lr = self.lr if lr is None else lr
         h = self._hyper
-        if list(map(_T.data_ptr, self._watched)) != self._at:
-            raise TeenyError(1, "a tensor has been given other memory: make a new AdamW with this one's state")
+        if self._addresses() != self._at:
+            raise TeenyError(1, "a tensor has been given other memory: make a new AdamW of the present ones")
         if isinstance(lr, torch.Tensor):
             h.lr, h.lr_dev = 0.0, self._scalar("lr", lr)
         elif lr >= 0:
@@ -806,8 +811,8 @@ class AdamW:
         else:
             raise TeenyError(1, f"lr must not be negative, got {lr}")
         h.grad_scale = None if grad_scale is None else self._scalar("grad_scale", grad_scale)
-        with _on(self.device) as ctx:
-            if torch.cuda.is_current_stream_capturing():
+        with (on := _on(self.device)) as ctx:
+            if on.stream and torch.cuda.is_current_stream_capturing():   # the default stream, 0, never is
                 if self._step_dev is None:
                     raise TeenyError(5, "a step whose count is on the host cannot be captured: AdamW(capturable=True)")
                 self._captured.append((lr, grad_scale))

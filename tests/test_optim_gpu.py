@@ -690,3 +690,30 @@ def test_grad_norm_of_sizes_whose_squares_f32_does_not_hold(dtype, size):
     # as test_grad_norm has it; a result under 2^-126 has steps of 2^-149
     assert abs(float(norm) - want) <= 18 * u.U32 * want + 2.0 ** -150
     assert abs(float(scale) - min(1.0, 1 / (want + 1e-6))) <= 20 * u.U32 / max(want, 1.0)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_refuses_moments_that_were_given_other_memory(bits):
+    ops(), error()
+    m = Model([300, 77], F32, F32, False, bits, seed=43)
+    for name in m.state:
+        o = m.optimiser()
+        o.step()
+        before = host(m.params[1])
+        kept = getattr(o, name)[1]
+        old = kept.data
+        kept.data = old.clone()            # as a restore may do
+        with pytest.raises(error(), match="other memory"):
+            o.step()
+        kept.data = old
+        o.step()                           # its own memory again
+        getattr(o, name)[1] = old.clone()  # another tensor in its place
+        with pytest.raises(error(), match="other memory"):
+            o.step()
+        assert o.step_count == 2
+        assert not np.array_equal(host(m.params[1]), before)
+    for name in ("params", "grads"):
+        o = m.optimiser()
+        getattr(o, name)[0] = getattr(o, name)[0].clone()
+        with pytest.raises(error(), match="other memory"):
+            o.step()
