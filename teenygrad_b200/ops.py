@@ -764,7 +764,8 @@ class AdamW:
         self._step_dev, self._step = None, step_count
         self._captured = []   # scalars that captured steps read at each replay
         if capturable:
-            self._step_dev = torch.full((1,), step_count, device=torch.device("cuda", self.device), dtype=torch.int64)
+            # the number of the step to come, so that it counts on behind a step that was launched
+            self._step_dev = torch.full((1,), step_count + 1, device=torch.device("cuda", self.device), dtype=torch.int64)
             self._hyper.step_dev = self._step_dev.data_ptr()
         if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1 and eps >= 0 and weight_decay >= 0):
             raise TeenyError(1, "betas in [0, 1), eps and weight_decay >= 0")
@@ -784,7 +785,7 @@ class AdamW:
     @property
     def step_count(self):
         """Steps taken (waits for the device when capturable)."""
-        return self._step if self._step_dev is None else int(self._step_dev)
+        return self._step if self._step_dev is None else int(self._step_dev) - 1
 
     def _addresses(self):
         at = []
@@ -816,8 +817,8 @@ class AdamW:
                 if self._step_dev is None:
                     raise TeenyError(5, "a step whose count is on the host cannot be captured: AdamW(capturable=True)")
                 self._captured.append((lr, grad_scale))
-            if self._step_dev is not None:
-                self._step_dev.add_(1)
             h.step = self._step + 1
             check(ctx, lib().tb_adamw_step(self._handle, ctypes.byref(h)))
+            if self._step_dev is not None:
+                self._step_dev.add_(1)
             self._step += 1

@@ -717,3 +717,21 @@ def test_adamw_refuses_moments_that_were_given_other_memory(bits):
         getattr(o, name)[0] = getattr(o, name)[0].clone()
         with pytest.raises(error(), match="other memory"):
             o.step()
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+def test_a_refused_step_is_not_counted(capturable):
+    ops()
+    a, b = (Model([300], F32, F32, False, 32, seed=44) for _ in range(2))
+    o, ref = a.optimiser(capturable=capturable, step_count=5), b.optimiser(step_count=5)
+    for x in (o, ref):
+        x.step()
+    o._hyper.eps = -1.0     # what the library refuses
+    for _ in range(3):
+        with pytest.raises(error()):
+            o.step()
+    assert o.step_count == 6
+    o._hyper.eps = EPS
+    for x in (o, ref):
+        x.step()
+    assert o.step_count == 7 and torch.equal(a.params[0], b.params[0])
