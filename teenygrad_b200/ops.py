@@ -806,17 +806,18 @@ class AdamW:
         if self._addresses() != self._at:
             raise TeenyError(1, "a tensor has been given other memory: make a new AdamW of the present ones")
         if isinstance(lr, torch.Tensor):
-            h.lr, h.lr_dev = 0.0, self._scalar("lr", lr)
+            rate, rate_dev = 0.0, self._scalar("lr", lr)
         elif lr >= 0:
-            h.lr, h.lr_dev = lr, None
+            rate, rate_dev = lr, None
         else:
             raise TeenyError(1, f"lr must not be negative, got {lr}")
-        h.grad_scale = None if grad_scale is None else self._scalar("grad_scale", grad_scale)
+        scale_dev = None if grad_scale is None else self._scalar("grad_scale", grad_scale)
         with (on := _on(self.device)) as ctx:
             if on.stream and torch.cuda.is_current_stream_capturing():   # the default stream, 0, never is
                 if self._step_dev is None:
                     raise TeenyError(5, "a step whose count is on the host cannot be captured: AdamW(capturable=True)")
                 self._captured.append((lr, grad_scale))
+            h.lr, h.lr_dev, h.grad_scale = rate, rate_dev, scale_dev
             h.step = self._step + 1
             check(ctx, lib().tb_adamw_step(self._handle, ctypes.byref(h)))
             if self._step_dev is not None:

@@ -118,3 +118,37 @@ def test_a_refused_call_lets_the_others_go_on(fake):
     t.start()
     t.join(10)
     assert done == [2] and not fake.bad
+
+
+def test_threads_that_step_one_optimiser_have_their_own_rates(fake, monkeypatch):
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    opt = object.__new__(ops.AdamW)
+    opt.__dict__.update(_handle=ctypes.c_void_p(1), _destroy=lambda h: 0, _hyper=ops._AdamWHyper(), _lists=(), _at=[], device=0,
+                        lr=1.0, _step=0, _step_dev=None, _captured=[], params=[], grads=[])
+    seen, errors = [], []
+
+    def step(handle, hyper):
+        first = (hyper._obj.lr, hyper._obj.step)
+        time.sleep(1e-4)
+        seen.append((fake.local.stream, *first, hyper._obj.lr))
+        return 0
+
+    fake.tb_adamw_step = step
+
+    def work(k):
+        fake.local.stream = 100 + k
+        try:
+            for _ in range(200):
+                opt.step(lr=100.0 + k)
+        except Exception as e:   # pragma: no cover - shown by the assertion
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    assert all(stream == lr == later for stream, lr, _, later in seen)
+    assert [n for _, _, n, _ in seen] == list(range(1, 601)) and opt.step_count == 600
+    opt._handle = None
