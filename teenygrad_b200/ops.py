@@ -708,7 +708,11 @@ class AdamW:
 
     capturable=True keeps the step count on the device, so that a captured step counts on at each
     replay; an lr given as a number is then the one of the capture, one given as an f32 CUDA tensor
-    of one element is read at each replay.  Without it a step cannot be captured."""
+    of one element is read at each replay.  Without it a step cannot be captured.  A graph with captured
+    steps must not outlive the optimiser, which holds the memory that they use.
+
+    What the constructor makes (moments of zeros, the count) is made on the current stream: a step on
+    another one has to come behind that."""
 
     def __init__(self, params, grads, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32,
                  copies=None, seed=0, state=None, step_count=0, capturable=False):
@@ -816,7 +820,8 @@ class AdamW:
             if on.stream and torch.cuda.is_current_stream_capturing():   # the default stream, 0, never is
                 if self._step_dev is None:
                     raise TeenyError(5, "a step whose count is on the host cannot be captured: AdamW(capturable=True)")
-                self._captured.append((lr, grad_scale))
+                # their memory, whatever becomes of the tensors
+                self._captured += [t.detach() for t in (lr, grad_scale) if isinstance(t, torch.Tensor)]
             h.lr, h.lr_dev, h.grad_scale = rate, rate_dev, scale_dev
             h.step = self._step + 1
             check(ctx, lib().tb_adamw_step(self._handle, ctypes.byref(h)))

@@ -735,3 +735,21 @@ def test_a_refused_step_is_not_counted(capturable):
     for x in (o, ref):
         x.step()
     assert o.step_count == 7 and torch.equal(a.params[0], b.params[0])
+
+
+def test_what_a_captured_step_reads_outlives_its_tensor():
+    """A learning rate and a scale that are given other memory after the capture: the graph reads what it was made with."""
+    ops()
+    a, b = (Model([3000], F32, F32, False, 32, seed=45) for _ in range(2))
+    lr, scale = torch.tensor([LR], device="cuda"), torch.tensor([0.25], device="cuda")
+    oa, ob = a.optimiser(capturable=True), b.optimiser()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        oa.step(lr=lr, grad_scale=scale)
+    lr.data, scale.data = torch.tensor([7.0], device="cuda"), torch.tensor([9.0], device="cuda")
+    others = [torch.full((1,), 5.0, device="cuda") for _ in range(64)]   # would take freed memory
+    for _ in range(2):
+        graph.replay()
+        ob.step(lr=LR, grad_scale=torch.tensor([0.25], device="cuda"))
+    torch.cuda.synchronize()
+    assert torch.equal(a.params[0], b.params[0]) and all(float(x) == 5 for x in others)
