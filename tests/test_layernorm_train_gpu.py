@@ -314,3 +314,40 @@ def test_refusals():
     assert l.tb_layernorm_fwd_train(ctx, 0, x.data_ptr(), w.data_ptr(), w.data_ptr(), dx.data_ptr(), dx.data_ptr(),
                                     rstd.data_ptr(), M, 8, 1e-5) == 1
     assert l.tb_layernorm_bwd(*args, dx.data_ptr(), ws.data_ptr(), db.data_ptr(), 0, M, 8, ws.data_ptr(), 1 << 20) == 1
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("M,N,odd", [(33, 264, True), (1000, 264, True), (1000, 2048, True), (47, 9001, True), (100, 8193, False),
+                                     (50, 12001, False), (40, 16384, True), (40, 16384, False)])
+def test_element_by_element_backward_in_several_splits(M, N, odd, accumulate, dtype):
+    """Tensors at odd addresses and long odd rows with more rows than one split takes: the partial sums stay in a
+    workspace of the size that is asked for, which is full of what another kernel left."""
+    import ctypes
+    o = ops()
+    from teenygrad_b200._lib import check, lib
+    bf16 = dtype == torch.bfloat16
+    x, w, _, dy = inputs(M, N, dtype, seed=9)
+    r = rng(2)
+
+    def at(a):
+        lead = 1 if odd else 0
+        t = torch.empty(a.size + lead, device="cuda", dtype=dtype)[lead:].view(a.shape)
+        return t.copy_(torch.from_numpy(np.ascontiguousarray(a)))
+
+    gx, gw, gdy = at(x), at(w), at(dy)
+    mean, rstd = to_gpu(x.mean(1)), to_gpu(1 / np.sqrt(x.astype(np.float64).var(1) + 1e-5))
+    dw0, db0 = (r.standard_normal(N).astype(np.float32) for _ in range(2))
+    dw, db, dx = to_gpu(dw0), to_gpu(db0), torch.empty_like(gx)
+    code, need = 1 if bf16 else 0, ctypes.c_size_t(0)
+    assert lib().tb_workspace_bytes(13, code, (ctypes.c_int64 * 2)(M, N), 2, ctypes.byref(need)) == 0
+    assert need.value >= 2 * 2 * N * 4
+    buf = torch.full((need.value + 512,), 0xFF, device="cuda", dtype=torch.uint8)   # NaN, as f32
+    ctx = o.context()
+    check(ctx, lib().tb_layernorm_bwd(ctx, code, gdy.data_ptr(), gx.data_ptr(), gw.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
+                                      dx.data_ptr(), dw.data_ptr(), db.data_ptr(), accumulate, M, N, buf.data_ptr() + 256,
+                                      need.value))
+    zero = np.zeros(N)
+    check_bwd(dy, x, w, f64(mean), f64(rstd), (dx, dw, db), bf16, *((dw0.astype(np.float64), db0.astype(np.float64)) if accumulate
+                                                                     else (zero, zero)))
+    assert bool((buf[:256] == 0xFF).all() and (buf[-256:] == 0xFF).all())
