@@ -92,6 +92,37 @@ def test_root_follows_a_falling_gradient():
     assert abs(np.mean(s / np.sqrt(v)) - 1) < 0.1
 
 
+@pytest.mark.parametrize("low,high,tol", [(1.0, 8.0, 0.012), (4 * 2.0 ** -9, 8 * 2.0 ** -9, 0.03)])
+def test_second_moment_is_high_by_the_roundings_variance(low, high, tol):
+    """The root is rounded without bias, so its square is high by the rounding's variance.
+
+    A step moves the root r by d = r (1 - b2) / 2 |g^2 / v - 1| from a code, and rounding back to that code or the next,
+    a step of the grid away, has the variance d step.  Where b2 v + (1 - b2) g^2 + d step stays v on the average, v is
+    1 / (1 - E|g^2 / v - 1| E[step / r] / 2) of the 32-bit one: for normal gradients E|g^2 / v - 1| = 4 phi(1) = 0.968, and
+    for sizes spread evenly over a binade of normal codes E[step / r] = 1 / (16 ln 2) = 0.0902: 4.6 % high.  Where codes are
+    k steps for k from 4 to 8 (the bottom of the range), E[step / r] = 1 / (8 ln 2): 9.6 %.  What is left out, the spread of
+    v itself (0.09 and 0.17 of it, squared deviations) and d against a step, is under a third of these."""
+    blocks, warm, T, b2 = 32, 400, 1000, 0.99
+    n = blocks * 256
+    r = np.random.default_rng(3)
+    size = np.exp(r.uniform(np.log(low), np.log(high), n)) / 8   # the exponent puts 16 at 128
+    first = np.arange(n) % 256 == 0
+    cm = cs = np.zeros(n, np.uint8)
+    em = es = np.zeros(blocks, np.uint8)
+    v, held, true = np.zeros(n), 0.0, 0.0
+    for t in range(1, warm + T + 1):
+        g = np.where(first, 16.0, r.standard_normal(n) * size).astype(np.float32)
+        cm, em, cs, es = u.adamw8_moments(g, cm, em, cs, es, 1, t, 0, 0.9, b2, 1.0)
+        v = b2 * v + (1 - b2) * g.astype(np.float64) ** 2
+        if t > warm:
+            held += np.mean((u.held(cs, es).astype(np.float64) ** 2 / size ** 2)[~first])
+            true += np.mean((v / size ** 2)[~first])
+    inverse = 1 / (np.log(2) * 16) if low == 1.0 else 1 / (np.log(2) * 8)
+    want = 1 / (1 - 4 * np.exp(-0.5) / np.sqrt(2 * np.pi) * inverse / 2)
+    # 8160 elements with 10 independent spells each: 0.42 / sqrt(81600) is 0.15 % of chance
+    assert abs(held / true - want) < tol, (held / true, want)
+
+
 def test_refuses_cpu_tensors():
     x, w = torch.ones(4, 8), torch.ones(8)
     one = torch.ones(4)
