@@ -8,13 +8,14 @@
 //
 // Bound by HBM: the forward moves x and y, the backward x, dy and dx, once
 // each.  A row belongs to a group of threads (a warp, or a CTA of as many as the
-// row needs), one or two 16-byte vectors a thread; the groups walk the rows with
-// the grid's stride and keep w (and b) in registers.  Each thread copies its own
-// vectors of the next rows into its own slots of a ring in shared memory
-// (cp.async: no registers, no barrier), so that rows are in flight while one is
-// reduced.  In the backward each thread also keeps the f32 sums of dw and db for
-// its columns over all the rows it walks; the CTAs write them as partial rows, and
-// a second launch adds those in CTA order: no atomics, the same bits on each run.
+// row needs), 16 elements a thread (two 16-byte vectors of bf16, four of f32); the
+// groups walk the rows with the grid's stride and keep w (and b) in registers.
+// Each thread copies its own vectors of the next rows into its own slots of a ring
+// in shared memory (cp.async: no registers, no barrier), so that rows are in flight
+// while one is reduced.  In the backward each thread also keeps the f32 sums of dw
+// and db for its columns over all the rows it walks; the CTAs write them as partial
+// rows, and a second launch adds those in CTA order: no atomics, the same bits on
+// each run.
 //
 // Rows whose length is no multiple of a vector start at any element.  Their
 // vectors are those of the tensor: the first may begin in the row before, the last

@@ -28,11 +28,14 @@
 //  * Each operation up to the code is rounded by itself (no fused multiply-add),
 //    so the codes are defined bit for bit by the formula.
 //
-// Measured over 1e9 parameters (the floor is the bytes at the rate of a copy, 6.45
-// TB/s): f32 moments, f32 parameters and gradients 4.37 ms (floor 4.34), bf16
-// gradients 4.12 (4.03), and a bf16 copy 4.55 (4.34), all bf16 3.50 (3.41); 8-bit
-// moments 2.74 (2.48), 2.67 (2.17), 2.62 (2.48) and 2.24 (1.55): there instruction
-// issue comes first, 56 of them an element.  1.1e9 bf16 gradients' norm 0.32 ms.
+// Measured over 1e9 parameters, steps back to back (the floor is the bytes at the rate
+// of a copy, 6.45 TB/s): f32 moments, f32 parameters and gradients 4.37 ms (floor 4.34),
+// bf16 gradients 4.14 (4.03), and a bf16 copy 4.65 (4.34), all bf16 3.56 (3.41); 8-bit
+// moments 2.76 (2.48), 2.62 (2.17), 2.81 (2.48) and 2.24 (1.55).  A step by itself, at the
+// highest clock, takes 2.47, 2.43, 2.54 and 2.18 ms with 8-bit moments: with f32 parameters
+// HBM is the bound there, and instruction issue (56 of them an element) at the clock that
+// steps back to back leave; with bf16 parameters issue is in both.  1.1e9 bf16 gradients'
+// norm 0.32 ms.
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <float.h>
@@ -199,9 +202,9 @@ __device__ __forceinline__ float stepped(float p, float m, float root_v, const S
     return p * s.keep - q;
 }
 
-// CTAs an SM: as many as keep HBM busy, since more of them cost DRAM rows.  1e9 parameters, with 2 / 3 / 4 CTAs:
-// f32 and f32 gradients 4.35 / 4.52 / 4.54 ms, bf16 gradients 4.72 / 4.12 / 4.28 and with the copy 5.01 / 4.55 / 4.62,
-// bf16 and bf16 4.38 / 3.70 / 3.50.  (The floors are 4.34, 4.03, 4.34 and 3.41.)
+// CTAs an SM: as many as keep HBM busy, since more of them cost DRAM rows.  1e9 parameters, back to back, with 2 / 3 / 4
+// CTAs: f32 and f32 gradients 4.37 / 4.65 / 4.70 ms, bf16 gradients 4.72 / 4.15 / 4.39 and with the copy 5.01 / 4.64 /
+// 4.78, bf16 and bf16 4.38 / 3.69 / 3.57.  (The floors are 4.34, 4.03, 4.34 and 3.41.)
 template <typename P, typename G>
 constexpr int adamw_ctas() {
     return sizeof(P) == 2 ? 4 : sizeof(G) == 2 ? 3 : 2;
@@ -538,12 +541,13 @@ __device__ __forceinline__ bool adamw8_unit(const UnitIn<P, G>& in, uint32_t exp
     return true;
 }
 
-// How many units a warp's ring holds and how many CTAs an SM.  With f32 parameters HBM is the
-// bound: 12 warps of 3 or 4 units (5 KB or 4 KB) keep enough in flight, and more of them cost
-// DRAM rows (1e9 parameters, bf16 gradients and a copy: 6 CTAs of 4 units 2.49 ms, 8 of 3 2.93,
-// 10 of 2 2.93, 4 of 4 3.09).  With bf16 parameters instruction issue is: as many warps as the
-// registers allow (10 CTAs of 2 units 1.99 ms, 6 of 4 2.31).  An odd number of CTAs leaves
-// sub-partitions of the SM uneven.
+// How many units a warp's ring holds and how many CTAs an SM.  With f32 parameters 12 warps
+// of 3 or 4 units (5 KB or 4 KB) keep enough in flight for HBM, and more of them cost DRAM
+// rows.  With bf16 parameters instruction issue is the bound: as many warps as the registers
+// allow.  1e9 parameters, a step by itself / back to back, ms: f32, bf16 gradients and a copy,
+// 6 CTAs of 4 units 2.54 / 2.81, 8 of 3 2.91 / 2.72, 10 of 2 2.96 / 2.99, 4 of 4 3.16 / 3.19;
+// all bf16, 10 CTAs of 2 units 2.18 / 2.24, 8 of 2 2.20 / 2.25, 10 of 3 2.24 / 2.30, 6 of 4
+// 2.39 / 2.35.  An odd number of CTAs leaves sub-partitions of the SM uneven.
 template <typename P, typename G>
 struct Ring8 {
     static constexpr bool wide = sizeof(P) == 4;
